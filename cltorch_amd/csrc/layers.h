@@ -1,0 +1,52 @@
+// Launches behind the layer operators (layer norm, linear layer, grouped products): what the entry points hand to the
+// kernels once shapes, views and aliasing are settled.  Pitches, steps and strides are in elements.
+#pragma once
+
+#include "internal.h"
+
+struct NormParams {
+  const float *x, *w, *b;
+  float *y, *mean, *rstd;
+  long rows, width, x_pitch, y_pitch, w_step, b_step;
+  float eps;
+};
+
+struct NormGradParams {
+  const float *gy, *x, *mean, *rstd, *w;
+  float *gx, *gw, *gb;
+  long rows, width, gy_pitch, x_pitch, gx_pitch, w_step, gw_step, gb_step;
+};
+
+void thcl_norm(THClState *state, thcl_rt *rt, const NormParams &P);
+void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &P);  // gx, gw, gb: NULL when not wanted
+
+enum ThclRagged : int { WHOLE = 0, ROWS = 1, DEPTH = 2 };
+
+// c(i, j) = sum over l of a(i, l) b(l, j), then the epilogue.  Strides are in elements; c has unit stride along j.
+// ROWS: the rows i lie group after group, and b moves on by b_g from group to group.  DEPTH: l does, and c moves on.
+struct Product {
+  const float *a, *b;
+  float *c;
+  long a_m, a_k, b_k, b_n, c_m;
+  int m, n, k;
+  const float *bias, *residual;
+  float *preact;
+  long bias_n, res_m, pre_m;
+  int act;
+  const float *sizes;  // rows of each group, as floats
+  int groups;
+  long b_g, c_g;
+  unsigned *fault;     // pinned word the host looks at after its next wait
+};
+
+void thcl_product(THClState *state, thcl_rt *rt, const Product &P, int ragged, const char *what);
+
+// gz = gy act'(z)
+struct SlopeParams {
+  const float *gy, *z;
+  float *gz;
+  long gy_pitch, z_pitch, gz_pitch;
+  long rows, width;
+  int act;
+};
+void thcl_activation_slope(THClState *state, thcl_rt *rt, const SlopeParams &P);

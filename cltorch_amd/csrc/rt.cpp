@@ -457,6 +457,11 @@ static int check_fault(thcl_rt *rt) {
             "the result of that scan is not valid";
     return -3;
   }
+  if (what == 3u) {
+    g_err = "group sizes out of range: a grouped product met sizes that are no whole numbers, are negative or come to more rows "
+            "than there are (that product wrote nothing)";
+    return -3;
+  }
   g_err = "index out of range: an indexing kernel met an index outside 1..size of the indexed dimension "
           "(that entry moved nothing; reported at the first wait after the launch)";
   return -3;

@@ -1039,6 +1039,30 @@ class ClTensor:
     def addr(self, *args) -> "ClTensor":
         return self._addblas("addr", args)
 
+    # ---- layers of a network -----------------------------------------------------
+    def layerNorm(self, src: "ClTensor", weight: Optional["ClTensor"] = None, bias: Optional["ClTensor"] = None, eps: float = 1e-5,
+                  mean: Optional["ClTensor"] = None, rstd: Optional["ClTensor"] = None) -> "ClTensor":
+        """``res:layerNorm(src, weight, bias, eps, mean, rstd)``: src normalised over its last dimension, times weight
+        plus bias.  ``mean`` and ``rstd`` receive the statistics that :func:`layerNormBackward` takes.  res may be src."""
+        _call("THClTensor_layerNorm", self._h, _handle_of(mean), _handle_of(rstd), src._h, _handle_of(weight), _handle_of(bias), C.c_float(eps))
+        return self
+
+    def linear(self, src: "ClTensor", weight: "ClTensor", bias: Optional["ClTensor"] = None, residual: Optional["ClTensor"] = None,
+               activation: str = "none", preact: Optional["ClTensor"] = None) -> "ClTensor":
+        """``res:linear(src, weight, bias, residual, activation, preact)``: activation(src * weight^T + bias) + residual
+        for src of ``[..., in]`` and weight of ``[out, in]``; activation is none, relu, gelu (the exact form) or silu.
+        ``preact`` receives the activation's input, which :func:`linearBackward` takes.  res may be residual."""
+        _call("THClTensor_linear", self._h, _handle_of(preact), src._h, weight._h, _handle_of(bias), _handle_of(residual), _activation(activation))
+        return self
+
+    def groupedmm(self, src: "ClTensor", weight: "ClTensor", sizes) -> "ClTensor":
+        """``res:groupedmm(src, weight, sizes)``: rows of src lie group after group, ``sizes[g]`` of them each, and are
+        multiplied by their group's matrix of weight ``[groups, in, out]``.  Rows of res behind the last group are left
+        as they were.  Sizes (a ClTensor, or a list of numbers) that do not fit the rows are reported by the next wait."""
+        sizes = _sizes_of(sizes)
+        _call("THClTensor_groupedmm", self._h, src._h, weight._h, sizes._h)
+        return self
+
     # ---- random fills (src/Random.lua:6-24): drawn on the host, then copied over ----------
     def uniform(self, a: float = 0.0, b: float = 1.0) -> "ClTensor":
         vals = _uniform01(self.nElement()) * (b - a) + a
@@ -1127,6 +1151,47 @@ class ClTensor:
 
     def __repr__(self):
         return f"ClTensor(size={self.size()}, stride={self.stride()})"
+
+
+_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # THCL_ACT_* of include/thcl_hip.h
+
+
+def _activation(name: str) -> int:
+    if name not in _ACTIVATIONS:
+        raise ClError(f"unknown activation {name!r}: none, relu, gelu or silu expected")
+    return _ACTIVATIONS[name]
+
+
+def _handle_of(t: Optional[ClTensor]):
+    return None if t is None else t._h
+
+
+def _sizes_of(sizes) -> ClTensor:
+    return sizes if isinstance(sizes, ClTensor) else ClTensor(np.asarray(sizes, dtype=np.float32).reshape(-1))
+
+
+def layerNormBackward(gradInput: Optional[ClTensor], gradWeight: Optional[ClTensor], gradBias: Optional[ClTensor], gradOutput: ClTensor,
+                      src: ClTensor, weight: Optional[ClTensor], mean: ClTensor, rstd: ClTensor) -> None:
+    """Gradients of :meth:`ClTensor.layerNorm` by its input, weight and bias into the first three tensors (None: not
+    wanted); ``mean`` and ``rstd`` are what the forward pass left.  gradInput may be gradOutput or src."""
+    _call("THClTensor_layerNormBackward", _handle_of(gradInput), _handle_of(gradWeight), _handle_of(gradBias), gradOutput._h, src._h,
+          mean._h, rstd._h, _handle_of(weight))
+
+
+def linearBackward(gradInput: Optional[ClTensor], gradWeight: Optional[ClTensor], gradBias: Optional[ClTensor], gradOutput: ClTensor,
+                   src: ClTensor, weight: ClTensor, preact: Optional[ClTensor] = None, activation: str = "none") -> None:
+    """Gradients of :meth:`ClTensor.linear` by its input, weight and bias into the first three tensors (None: not
+    wanted); the residual's is gradOutput itself.  ``preact`` is what the forward pass left, needed with an activation."""
+    _call("THClTensor_linearBackward", _handle_of(gradInput), _handle_of(gradWeight), _handle_of(gradBias), gradOutput._h, src._h,
+          weight._h, _handle_of(preact), _activation(activation))
+
+
+def groupedmmBackward(gradInput: Optional[ClTensor], gradWeight: Optional[ClTensor], gradOutput: ClTensor, src: ClTensor,
+                      weight: ClTensor, sizes) -> None:
+    """Gradients of :meth:`ClTensor.groupedmm` by its rows (those behind the last group are left as they were) and by
+    the groups' matrices (zero for a group without rows) into the first two tensors (None: not wanted)."""
+    sizes = _sizes_of(sizes)
+    _call("THClTensor_groupedmmBackward", _handle_of(gradInput), _handle_of(gradWeight), gradOutput._h, src._h, weight._h, sizes._h)
 
 
 def mm(a: ClTensor, b: ClTensor) -> ClTensor:

@@ -544,6 +544,41 @@ void THClBlas_ger(THClState *state, long m, long n, float alpha, THClTensor *x, 
                   THClTensor *a, long lda);
 
 /* ------------------------------------------------------------------------- */
+/* Layers of a network (no counterpart in the reference, whose users compose   */
+/* them from addmm, sum and the pointwise operators).  Results are resized;    */
+/* they must not share memory with an operand unless said otherwise.  NULL     */
+/* stands for an operand or a result that is not there.                        */
+/* ------------------------------------------------------------------------- */
+/* Layer norm over the last dimension: self = (src - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps);
+ * weight and bias are vectors or NULL (1 and 0).  mean and rstd, of src's shape without its last dimension, keep the
+ * statistics for the backward pass, or are NULL.  self may be src. */
+void THClTensor_layerNorm(THClState *state, THClTensor *self, THClTensor *mean, THClTensor *rstd, THClTensor *src,
+                          THClTensor *weight, THClTensor *bias, float eps);
+/* Gradients by the input, the weight and the bias, each or NULL.  gradInput may be gradOutput or src. */
+void THClTensor_layerNormBackward(THClState *state, THClTensor *gradInput, THClTensor *gradWeight, THClTensor *gradBias,
+                                  THClTensor *gradOutput, THClTensor *src, THClTensor *mean, THClTensor *rstd,
+                                  THClTensor *weight);
+enum { THCL_ACT_NONE = 0, THCL_ACT_RELU = 1, THCL_ACT_GELU = 2, THCL_ACT_SILU = 3 };
+/* self = act(src * weight^T + bias) + residual; src [..., in], weight [out, in], bias [out] or NULL, residual
+ * [..., out] or NULL.  preact keeps src * weight^T + bias for the backward pass, or is NULL.  self may be residual. */
+void THClTensor_linear(THClState *state, THClTensor *self, THClTensor *preact, THClTensor *src, THClTensor *weight,
+                       THClTensor *bias, THClTensor *residual, int activation);
+/* Gradients by the input, the weight and the bias, each or NULL (the residual's is gradOutput itself).  preact is
+ * what the forward pass kept; it is not looked at for THCL_ACT_NONE.  relu passes nothing on at 0. */
+void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTensor *gradWeight, THClTensor *gradBias,
+                               THClTensor *gradOutput, THClTensor *src, THClTensor *weight, THClTensor *preact,
+                               int activation);
+/* Rows of src [rows, in] lie group after group, sizes[g] of them each: every row is multiplied by its group's matrix
+ * of weight [groups, in, out].  sizes is a vector of whole numbers as floats (below 2^24 each).  Rows behind the last
+ * group are left as they were.  Sizes that are negative, no whole numbers or come to more than the rows make the call
+ * write nothing; the next call that waits for the stream reports it, as for an index out of range. */
+void THClTensor_groupedmm(THClState *state, THClTensor *self, THClTensor *src, THClTensor *weight, THClTensor *sizes);
+/* Gradients by src (rows behind the last group are left as they were) and by weight (zero for a group without rows),
+ * each or NULL. */
+void THClTensor_groupedmmBackward(THClState *state, THClTensor *gradInput, THClTensor *gradWeight, THClTensor *gradOutput,
+                                  THClTensor *src, THClTensor *weight, THClTensor *sizes);
+
+/* ------------------------------------------------------------------------- */
 /* Indexed movement (reference: src/lib/THClTensorMath.h:101-116,130-132).     */
 /* Index tensors hold 1-based positions as floats; `dim` is 0-based.  An       */
 /* index outside the dimension moves nothing.                                  */
