@@ -225,7 +225,7 @@ void THClTensor_linear(THClState *state, THClTensor *self, THClTensor *preact, T
     z.emplace(state, preact);
     P.preact = z->p, P.pre_m = z->pitch;
   }
-  thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, WHOLE, "linear");
+  thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linear");
   if (z) z->finish();
   y.finish();
   THCL_GUARD_END()
@@ -284,7 +284,7 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
     P.b = w.p, P.b_k = w.s0, P.b_n = w.s1;
     P.c = gx.p, P.c_m = gx.pitch;
     P.m = (int)M, P.n = (int)K, P.k = (int)N;
-    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, WHOLE, "linearBackward");
+    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linearBackward");
     gx.finish();
   }
   if (gradWeight) {
@@ -294,7 +294,7 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
     P.b = x.p, P.b_k = x.pitch, P.b_n = 1;
     P.c = gw.p, P.c_m = gw.pitch;
     P.m = (int)N, P.n = (int)K, P.k = (int)M;
-    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, WHOLE, "linearBackward");
+    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linearBackward");
     gw.finish();
   }
   if (gradBias) {
@@ -345,8 +345,9 @@ void THClTensor_groupedmm(THClState *state, THClTensor *self, THClTensor *src, T
   P.m = (int)T, P.n = (int)N, P.k = (int)K;
   P.sizes = thcl_dptr(s.t);
   P.groups = (int)G;
+  P.ragged = ROWS;
   P.fault = thcl_rt_fault_word_device(rt);
-  thcl_product(state, rt, P, ROWS, "groupedmm");
+  thcl_product(state, rt, P, "groupedmm");
   if (dense.t) dense.give_to(self);
   THCL_GUARD_END()
 }
@@ -396,8 +397,9 @@ void THClTensor_groupedmmBackward(THClState *state, THClTensor *gradInput, THClT
     P.m = (int)K, P.n = (int)N, P.k = (int)T;
     P.sizes = thcl_dptr(s.t);
     P.groups = (int)G;
+    P.ragged = DEPTH;
     P.fault = thcl_rt_fault_word_device(rt);
-    thcl_product(state, rt, P, DEPTH, "groupedmmBackward");
+    thcl_product(state, rt, P, "groupedmmBackward");
     if (dense.t) dense.give_to(gradWeight);
   }
   THCL_GUARD_END()

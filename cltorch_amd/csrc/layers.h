@@ -35,11 +35,15 @@ struct Product {
   int act;
   const float *sizes;  // rows of each group, as floats
   int groups;
+  int ragged;          // ThclRagged
   long b_g, c_g;
   unsigned *fault;     // pinned word the host looks at after its next wait
+  // set by thcl_product: k cut into slices, whose partial results lie in work as [slice][group][m][n]
+  int slices;
+  float *work;
 };
 
-void thcl_product(THClState *state, thcl_rt *rt, const Product &P, int ragged, const char *what);
+void thcl_product(THClState *state, thcl_rt *rt, const Product &P, const char *what);
 
 // gz = gy act'(z)
 struct SlopeParams {

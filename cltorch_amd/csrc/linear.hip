@@ -7,7 +7,9 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "layers.h"
 
@@ -37,13 +39,19 @@ __device__ __forceinline__ float activation_slope(int act, float z) {
   return 1.f;
 }
 
-__device__ __forceinline__ void finish(const Product &P, float *c, int row, int col, float v) {
-  if (P.bias) v += P.bias[col * P.bias_n];
-  if (P.preact) P.preact[row * P.pre_m + col] = v;
-  v = activation(P.act, v);
-  if (P.residual) v += P.residual[row * P.res_m + col];
-  c[row * P.c_m + col] = v;
-}
+// the epilogue of one column of the result
+struct Column {
+  int col;
+  float bias;
+  __device__ __forceinline__ Column(const Product &P, int c) : col(c), bias(P.bias ? P.bias[c * P.bias_n] : 0.f) {}
+  __device__ __forceinline__ void finish(const Product &P, float *c, int row, float v) const {
+    const float res = P.residual ? P.residual[row * P.res_m + col] : 0.f;
+    v += bias;
+    if (P.preact) P.preact[row * P.pre_m + col] = v;
+    v = activation(P.act, v) + res;
+    c[row * P.c_m + col] = v;
+  }
+};
 
 // ------------------------------------------------------------------ groups ---
 // Where a block's work lies, worked out from the sizes by every wave for itself: lanes take 64 groups at a time and
@@ -61,6 +69,23 @@ __device__ __forceinline__ long wave_scan(long v, int lane) {
     if (lane >= d) v += below;
   }
   return v;
+}
+
+// rows of all groups together
+__device__ __forceinline__ long count_rows(const float *sizes, int groups, int total, bool &valid) {
+  long rows = 0;
+  valid = true;
+  for (int g0 = 0; g0 < groups && valid; g0 += kWave) {
+    const int g = g0 + threadIdx.x % kWave;
+    const float s = g < groups ? sizes[g] : 0.f;
+    valid = !__any(!(s >= 0.f && s <= (float)total && s == floorf(s)));
+    long n = valid ? (long)s : 0;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) n += __shfl_xor(n, d, kWave);
+    rows += n;
+    valid = valid && rows <= total;
+  }
+  return rows;
 }
 
 // want: a tile of `tile` rows counted over all groups (tile > 0), or a group (tile == 0)
@@ -100,74 +125,399 @@ __device__ __forceinline__ Place locate(const float *sizes, int groups, int tota
 }
 
 // ----------------------------------------------------------------- product ---
-// A wave's MT x NT tiles of 32 x 32 straight from memory, one v_mfma_f32_32x32x2_f32 per tile and two values of k:
-// lanes 0-31 hold k, lanes 32-63 k + 1.  Addresses beyond the matrix are moved to its last line, whose results are
-// not stored; beyond the last k both operands read as zero.
-template <int MT, int NT>
-__device__ __forceinline__ void product_direct(f16v (&acc)[MT][NT], const float *a, long a_m, long a_k, int m, const float *b, long b_n,
-                                               long b_k, int n, int row0, int col0, int k0, int k1) {
+// A tile of 32 x 32 straight from memory, one v_mfma_f32_32x32x2_f32 for two values of k: lanes 0-31 hold k, lanes
+// 32-63 k + 1.  Line i is line row0 + row_step i (col0 + col_step i).  Addresses beyond the matrix are moved to its
+// last line, whose results are not stored; beyond the last k both operands read as zero.
+__device__ __forceinline__ f16v product_direct(const float *a, long a_m, long a_k, int m, const float *b, long b_n, long b_k, int n,
+                                               int row0, int row_step, int col0, int col_step, int k0, int k1) {
   const int lane = threadIdx.x % kWave, l32 = lane % 32, h = lane / 32;
-  const float *ap[MT], *bp[NT];
+  const float *ap = a + (long)min(row0 + row_step * l32, m - 1) * a_m;
+  const float *bp = b + (long)min(col0 + col_step * l32, n - 1) * b_n;
+  constexpr int FLY = 8;
+  f16v acc = {};
+  for (int kk = k0; kk < k1; kk += 2 * FLY) {
+    float av[FLY], bv[FLY];
 #pragma unroll
-  for (int i = 0; i < MT; i++) ap[i] = a + (long)min(row0 + 32 * i + l32, m - 1) * a_m;
+    for (int f = 0; f < FLY; f++) {
+      const long k = min(kk + 2 * f + h, k1 - 1);
+      av[f] = ap[k * a_k];
+      bv[f] = bp[k * b_k];
+    }
 #pragma unroll
-  for (int j = 0; j < NT; j++) bp[j] = b + (long)min(col0 + 32 * j + l32, n - 1) * b_n;
-  for (int kk = k0; kk < k1; kk += 2) {
-    const int k = kk + h, kc = min(k, k1 - 1);
-    const bool in = k < k1;
-    float av[MT], bv[NT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) av[i] = ap[i][(long)kc * a_k];
-#pragma unroll
-    for (int j = 0; j < NT; j++) bv[j] = bp[j][(long)kc * b_k];
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? av[i] : 0.f, in ? bv[j] : 0.f, acc[i][j], 0, 0, 0);
+    for (int f = 0; f < FLY; f++) {
+      const bool in = kk + 2 * f + h < k1;
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? av[f] : 0.f, in ? bv[f] : 0.f, acc, 0, 0, 0);
+    }
   }
+  return acc;
 }
 
-constexpr int BM = 64, BN = 128, THREADS = 256;
+// A value that is the same in every lane, which the compiler has to be told: descriptors and loop counts live in
+// scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v) {
+  return (long)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
 
-template <int RAGGED>
-__global__ __launch_bounds__(THREADS) void product_tiles(Product P) {
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  int row0 = blockIdx.x * BM, rows = P.m, k0 = 0, k1 = P.k;
-  const float *b = P.b;
-  float *c = P.c;
-  if (RAGGED != WHOLE) {
-    bool valid;
-    const int want = RAGGED == ROWS ? blockIdx.x : blockIdx.z;
-    const Place at = locate(P.sizes, P.groups, RAGGED == ROWS ? P.m : P.k, RAGGED == ROWS ? BM : 0, want, valid);
-    if (!valid) {
-      if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) *P.fault = kFaultGroups;
-      return;
-    }
-    if (at.group < 0) return;
-    if (RAGGED == ROWS) {
-      row0 = at.first;
-      rows = at.first + at.count;
-      b += at.group * P.b_g;
-    } else {
-      k0 = at.first;
-      k1 = at.first + at.count;
-      c += at.group * P.c_g;
-    }
+// What a block works on, the same for every kernel below: rows [row0, rows) and columns [col0, n) of a product over
+// k in [k0, k1).  false: nothing, or sizes that do not fit.
+struct Work {
+  const float *b;
+  float *c;
+  int row0, rows, k0, k1;
+  int group;
+};
+__device__ __forceinline__ bool find_work(const Product &P, int tile_rows, int row_tile, int group, bool first_block, Work &w) {
+  w.b = P.b;
+  w.c = P.c;
+  w.row0 = row_tile * tile_rows;
+  w.rows = P.m;
+  w.k0 = 0;
+  w.k1 = P.k;
+  w.group = 0;
+  if (P.ragged == WHOLE) return w.row0 < w.rows;
+  bool valid;
+  const bool by_rows = P.ragged == ROWS;
+  const Place at = locate(P.sizes, P.groups, by_rows ? P.m : P.k, by_rows ? tile_rows : 0, by_rows ? row_tile : group, valid);
+  if (!uniform((int)valid)) {
+    if (threadIdx.x == 0 && first_block) *P.fault = kFaultGroups;
+    return false;
   }
-  row0 += (wave / 2) * 32;
-  const int col0 = blockIdx.y * BN + (wave % 2) * 64;
-  if (row0 >= rows || col0 >= P.n) return;
-  f16v acc[1][2] = {};
-  product_direct<1, 2>(acc, P.a, P.a_m, P.a_k, rows, b, P.b_n, P.b_k, P.n, row0, col0, k0, k1);
-#pragma unroll
+  const int group_at = uniform(at.group), first = uniform(at.first), count = uniform(at.count);
+  if (group_at < 0) return false;
+  if (by_rows) {
+    w.row0 = first;
+    w.rows = first + count;
+    w.b += group_at * P.b_g;
+  } else {
+    w.k0 = first;
+    w.k1 = first + count;
+    w.c += group_at * P.c_g;
+    w.group = group_at;
+  }
+  return true;
+}
+
+// Products whose pitches are too long for the tiled kernel's 32-bit offsets.
+constexpr int kDirectM = 64, kDirectN = 128;
+__global__ __launch_bounds__(256) void product_far(Product P) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  Work w;
+  if (!find_work(P, kDirectM, blockIdx.x, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0, w)) return;
+  const int row0 = w.row0 + (wave / 2) * 32, col0 = blockIdx.y * kDirectN + (wave % 2) * 64;
+  if (row0 >= w.rows || col0 >= P.n) return;
+#pragma unroll 1
   for (int j = 0; j < 2; j++) {
+    const f16v acc = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0, 1, col0 + 32 * j, 1, w.k0, w.k1);
     const int col = col0 + 32 * j + lane % 32;
     if (col >= P.n) continue;
+    const Column line(P, col);
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-      if (row < rows) finish(P, c, row, col, acc[0][j][r]);
+      if (row < w.rows) line.finish(P, w.c, row, acc[r]);
     }
+  }
+}
+
+// ------------------------------------------------------- fp32 on the bf16 pipes ---
+// The chip multiplies bf16 matrices 16 times as fast as fp32 ones.  Each fp32 value is written as the sum of three
+// bf16 values, x = h + m + l, each rounded to nearest from what the ones before leave: 8 significant bits each and
+// the signs of the remainders make up all 24 of x.  Of the nine products of two such sums six are taken, lh, hl, mm,
+// mh, hm, hh; the dropped ones are below 2^-25 of the whole, half of fp32's own rounding of a product.  Products of
+// bf16 values are exact in fp32, and the matrix instructions add them to fp32 accumulators.
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+
+constexpr int KS = 16;      // k per slab: two chunks of 8, one matrix instruction deep
+constexpr int CHUNKS = KS / 8;
+
+__device__ __forceinline__ unsigned round_pair(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, bf2)); }
+
+__device__ __forceinline__ void split_octet(const float (&x)[8], u4 (&part)[3]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+      const unsigned v = round_pair(a, b);
+      part[p][i] = v;
+      a -= __uint_as_float(v << 16);
+      b -= __uint_as_float(v & 0xffff0000u);
+    }
+  }
+}
+
+// One operand's part of a slab in LDS: [part][chunk of 8 k][line], 16 bytes each, so that a matrix instruction's
+// fragment (32 lines of one chunk in lanes 0-31, of the next in lanes 32-63) is read in one piece.  The lines of a
+// wave are dealt out to its IL tiles in turn (tile t has lines IL i + t), which gives a lane neighbouring columns of
+// the result.  The paddings keep the eight lanes of a 16-byte store phase on different banks, for lanes that hold
+// four lines of two chunks as well as for lanes that hold eight lines.
+template <int LINES, int IL>
+struct Staged {
+  static constexpr int TILES = LINES / 32;
+  static constexpr int TS = IL == 4 ? 544 : IL == 2 ? 576 : 512;
+  static constexpr int CP = (TILES * TS + 127) / 128 * 128 + (IL == 4 ? 16 : IL == 2 ? 32 : 64);
+  static constexpr int PART = CHUNKS * CP;
+  static constexpr int BYTES = 3 * PART;
+  static __device__ __forceinline__ int at(int line, int chunk) {
+    const int w = line / (32 * IL), r = line % (32 * IL);
+    return chunk * CP + (w * IL + r % IL) * TS + (r / IL) * 16;
+  }
+};
+
+// An operand on its way to LDS.  KC: contiguous along k (lanes take octets of k of a line, two lanes a line);
+// otherwise contiguous along its lines (lanes take neighbouring lines, eight k each).  Loads go through a buffer
+// descriptor that begins at the slab and ends behind the last element, so what lies behind reads as zero.
+template <int LINES, int IL, bool KC, int TH>
+struct Feed {
+  typedef Staged<LINES, IL> S;
+  static constexpr int OCTETS = LINES * CHUNKS;
+  static constexpr int N = OCTETS >= TH ? OCTETS / TH : 1;
+  const char *base;       // the slab that is loaded next
+  long left;              // bytes from there to behind the last element; what is not positive reads as zero
+  long step;
+  unsigned off[N];
+  int row_bytes;          // along k, when the lines are contiguous
+  int to[N];              // where the octet goes in LDS
+  unsigned least = ~0u;   // smallest magnitude met: its bits shifted up by one, less one (zero counts as the largest)
+  __device__ __forceinline__ void begin(const float *p, long line_stride, long k_stride, int line0, int lines, int k0, int k1) {
+    const long have = min(lines - line0, LINES);
+    base = (const char *)uniform((long)(p + (long)line0 * line_stride + (long)k0 * k_stride));
+    left = uniform(4 * ((have - 1) * line_stride + (long)(k1 - k0 - 1) * k_stride + 1));
+    step = 4 * KS * k_stride;
+    row_bytes = (int)(4 * k_stride);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int f = (threadIdx.x + TH * i) % OCTETS;  // threads beyond the last octet repeat one: no branch around loads
+      const int line = KC ? f / CHUNKS : f % LINES, chunk = KC ? f % CHUNKS : f / LINES;
+      off[i] = (unsigned)(4 * (line * line_stride + 8l * chunk * k_stride));
+      to[i] = S::at(line, chunk);
+    }
+  }
+  __device__ __forceinline__ void load(float (&x)[N][8]) {
+    const long l = left < 0 ? 0 : left > 0xffffffffl ? 0xffffffffl : left;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)l, 0x00020000);
+    base += step;
+    left -= step;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (KC) {
+        const f4 a = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i], 0, 0));
+        const f4 b = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i] + 16, 0, 0));
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off[i], e * row_bytes, 0));
+      }
+    }
+  }
+  // LAST: kleft values of k from the slab's first on are the operand's; those behind belong to the next line
+  template <bool LAST>
+  __device__ __forceinline__ void store(char *lds, float (&x)[N][8], int kleft) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (KC && LAST) {
+        const int chunk = (threadIdx.x + TH * i) % CHUNKS;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = 8 * chunk + e < kleft ? x[i][e] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) least = min(least, (__float_as_uint(x[i][e]) << 1) - 1u);
+      u4 part[3];
+      split_octet(x[i], part);
+#pragma unroll
+      for (int p = 0; p < 3; p++) *(u4 *)(lds + to[i] + p * S::PART) = part[p];
+    }
+  }
+};
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, TH = 64 * WM * WN;
+  static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
+  static constexpr int LDS = Staged<BM, MT>::BYTES + Staged<BN, NT>::BYTES;
+};
+
+// logical tile id -> tile coordinates.  Blocks go to the 8 XCDs in turn, and each XCD has its own L2: its blocks get
+// neighbouring ids, and ids walk 8 tiles down the rows before they step along the columns.
+__device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tiles_n, int &tm, int &tn) {
+  const int xcd = id % 8, q = total / 8, r = total % 8;
+  const int lid = xcd * q + min(xcd, r) + id / 8;
+  const int per = 8 * tiles_n, g = lid / per, in = lid % per;
+  const int down = min(tiles_m - 8 * g, 8);
+  tm = 8 * g + in % down;
+  tn = in / down;
+}
+
+template <class T, bool AKC, bool BKC>
+__global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m, int tiles_n) {
+  constexpr int MT = T::MT, NT = T::NT;
+  typedef Feed<T::BM, MT, AKC, T::TH> FA;
+  typedef Feed<T::BN, NT, BKC, T::TH> FB;
+  typedef Staged<T::BM, MT> SA;
+  typedef Staged<T::BN, NT> SB;
+  __shared__ __attribute__((aligned(16))) char lds[2][T::LDS];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+  Work w;
+  if (!find_work(P, T::BM, tm, blockIdx.y, blockIdx.x == 0 && blockIdx.y == 0, w)) return;
+  const int col0 = tn * T::BN;
+  if (P.slices > 1) {  // this block's slice of k, whole slabs
+    const int per = ((w.k1 - w.k0 + P.slices - 1) / P.slices + KS - 1) / KS * KS;
+    w.k0 = min(w.k0 + (int)blockIdx.z * per, w.k1);
+    w.k1 = min(w.k0 + per, w.k1);
+  }
+
+  FA fa;
+  FB fb;
+  fa.begin(P.a, P.a_m, P.a_k, w.row0, w.rows, w.k0, w.k1);
+  fb.begin(w.b, P.b_n, P.b_k, col0, P.n, w.k0, w.k1);
+  const int depth = w.k1 - w.k0, slabs = (depth + KS - 1) / KS;
+  float xa[2][FA::N][8], xb[2][FB::N][8];
+  f16v acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) acc[i][j] = f16v{};
+
+  const int frag = (lane / 32) * 1, l16 = (lane % 32) * 16;
+  const char *la = &lds[0][0] + frag * SA::CP + (wave / T::WN) * MT * SA::TS + l16;
+  const char *lb = &lds[0][0] + SA::BYTES + frag * SB::CP + (wave % T::WN) * NT * SB::TS + l16;
+
+  // Slab s is multiplied from one half of LDS while slab s + 1 is split into the other and slab s + 2 is on its way.
+  auto fill = [&](auto last, int set, int half, int s) {
+    fa.template store<decltype(last)::value>(lds[half], xa[set], depth - s * KS);
+    fb.template store<decltype(last)::value>(lds[half] + SA::BYTES, xb[set], depth - s * KS);
+  };
+  auto fetch = [&](int set) {
+    fa.load(xa[set]);
+    fb.load(xb[set]);
+  };
+  auto multiply = [&](int half) {
+    bf8 b[NT][3];
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int p = 0; p < 3; p++) b[j][p] = *(const bf8 *)(lb + half * T::LDS + p * SB::PART + j * SB::TS);
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      bf8 a[3];
+#pragma unroll
+      for (int p = 0; p < 3; p++) a[p] = *(const bf8 *)(la + half * T::LDS + p * SA::PART + i * SA::TS);
+      constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+      for (int q = 0; q < 6; q++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa[q]], b[j][pb[q]], acc[i][j], 0, 0, 0);
+    }
+  };
+  if (slabs > 0) {
+    const std::false_type whole;
+    const std::true_type last;
+    fetch(0);
+    fetch(1);
+    fill(last, 0, 0, 0);
+    __syncthreads();
+    fetch(0);
+    int s = 0;
+    // per turn: slab s from half 0, slab s + 1 from half 1; set 1 holds slab s + 1, set 0 slab s + 2
+    for (; s + 3 < slabs; s += 2) {
+      fill(whole, 1, 1, s + 1);
+      fetch(1);
+      multiply(0);
+      __syncthreads();
+      fill(whole, 0, 0, s + 2);
+      fetch(0);
+      multiply(1);
+      __syncthreads();
+    }
+    // the last one to three
+    if (s + 1 < slabs) fill(last, 1, 1, s + 1);
+    multiply(0);
+    if (s + 1 < slabs) {
+      __syncthreads();
+      if (s + 2 < slabs) fill(last, 0, 0, s + 2);
+      multiply(1);
+    }
+    if (s + 2 < slabs) {
+      __syncthreads();
+      multiply(0);
+    }
+  }
+
+  // What does not split is taken again with fp32 products.  A value that is not finite (or rounds to an infinity) leaves
+  // NaN among its parts, which shows in every result it belongs to; the others stay as they are.  A value below 2^-110
+  // has bits below bf16's smallest, 2^-133; the staging threads have looked out for those.
+  const bool tiny = __syncthreads_or(min(fa.least, fb.least) < (17u << 24) - 1u);  // and LDS is taken for the results below
+  const int row0 = w.row0 + (wave / T::WN) * 32 * MT, wcol0 = col0 + (wave % T::WN) * 32 * NT;
+  if (row0 >= w.rows || wcol0 >= P.n) return;
+  const int colb = wcol0 + NT * (lane % 32);
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      bool again = tiny;
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        again |= row0 + MT * (8 * (r / 4) + 4 * (lane / 32) + r % 4) + i < w.rows && colb + j < P.n && !(fabsf(acc[i][j][r]) < INFINITY);
+      if (__any(again)) {
+        const f16v v = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0 + i, MT, wcol0 + j, NT, w.k0, w.k1);
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][j][r] = tiny || !(fabsf(acc[i][j][r]) < INFINITY) ? v[r] : acc[i][j][r];
+      }
+    }
+  // 32 rows at a time through the wave's own part of LDS, so that a lane keeps one column and a wave stores whole rows
+  constexpr int COLS = 32 * NT, PER = kWave / COLS > 0 ? kWave / COLS : 1, LANES = COLS < kWave ? COLS : kWave;
+  static_assert(COLS <= kWave && 4 * 32 * COLS * T::WM * T::WN <= 2 * T::LDS, "a wave's rows fit its part of LDS");
+  float *mine = (float *)&lds[0][0] + wave * 32 * COLS;
+  const int col = wcol0 + lane % LANES;
+  const Column line(P, min(col, P.n - 1));
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) mine[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * COLS + NT * (lane % 32) + j] = acc[i][j][r];
+    if (col < P.n) {
+      float *part = P.slices > 1 ? P.work + (((long)blockIdx.z * gridDim.y + w.group) * P.m) * P.n + col : nullptr;
+      for (int q = lane / LANES; q < 32; q += PER) {
+        const int row = row0 + MT * q + i;
+        const float v = mine[q * COLS + lane % LANES];
+        if (row < w.rows) {
+          if (part) part[(long)row * P.n] = v;
+          else line.finish(P, w.c, row, v);
+        }
+      }
+    }
+  }
+}
+
+// The slices of k of every result, added in order, and the epilogue.
+template <int VEC>
+__global__ __launch_bounds__(256) void add_slices(Product P, int groups) {
+  int rows = P.m;
+  if (P.ragged != WHOLE) {
+    bool valid;
+    const long total = count_rows(P.sizes, P.groups, P.ragged == ROWS ? P.m : P.k, valid);
+    if (!valid) return;
+    if (P.ragged == ROWS) rows = (int)total;
+  }
+  const long per = (long)P.m * P.n, units = P.n / VEC, all = (long)groups * rows * units;
+  for (long u = (long)blockIdx.x * 256 + threadIdx.x; u < all; u += (long)gridDim.x * 256) {
+    const long line = u / units;
+    const int col = (int)(u % units) * VEC, row = (int)(line % rows), g = (int)(line / rows);
+    const float *p = P.work + g * per + (long)row * P.n + col;
+    typedef float V __attribute__((ext_vector_type(VEC)));
+    V sum = *(const V *)p;
+    for (int s = 1; s < P.slices; s++) sum += *(const V *)(p + (long)s * groups * per);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) Column(P, col + e).finish(P, P.c + g * P.c_g, row, sum[e]);
   }
 }
 
@@ -182,23 +532,63 @@ __global__ __launch_bounds__(256) void slope_rows(SlopeParams P) {
 }
 
 
+// an operand's pitch from which a tile's lines no longer fit 32-bit byte offsets
+constexpr long kFarPitch = 1l << 21;
+
 void check_launch(const char *what) {
   const hipError_t e = hipGetLastError();
   THCL_CHECK(e == hipSuccess, "%s launch failed: %s", what, hipGetErrorString(e));
 }
 }  // namespace
 
-void thcl_product(THClState *state, thcl_rt *rt, const Product &P, int ragged, const char *what) {
+template <class T>
+static void launch_split(const Product &P, bool akc, bool bkc, hipStream_t stream) {
+  const int tiles_n = (P.n + T::BN - 1) / T::BN;
+  int tiles_m = (P.m + T::BM - 1) / T::BM;
+  if (P.ragged == ROWS) tiles_m = P.m / T::BM + (P.groups < P.m ? P.groups : P.m);
+  THCL_CHECK((long)tiles_m * tiles_n <= INT32_MAX && P.groups <= 65535, THCL_DIM_WARNING);
+  const dim3 grid((unsigned)(tiles_m * tiles_n), P.ragged == DEPTH ? P.groups : 1, P.slices), block(T::TH);
+  if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true>), grid, block, 0, stream, P, tiles_m, tiles_n);
+  else if (akc) hipLaunchKernelGGL((product_split<T, true, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
+  else hipLaunchKernelGGL((product_split<T, false, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
+}
+
+void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const char *what) {
   hipStream_t stream = (hipStream_t)thcl_rt_stream(rt);
-  const unsigned gy = (unsigned)((P.n + BN - 1) / BN);
-  unsigned gx = (unsigned)((P.m + BM - 1) / BM), gz = 1;
-  if (ragged == ROWS) gx = (unsigned)(P.m / BM + (P.groups < P.m ? P.groups : P.m));
-  if (ragged == DEPTH) gz = (unsigned)P.groups;
-  THCL_CHECK(gy <= 65535 && gz <= 65535, THCL_DIM_WARNING);
-  const dim3 grid(gx, gy, gz), block(THREADS);
-  if (ragged == WHOLE) hipLaunchKernelGGL(product_tiles<WHOLE>, grid, block, 0, stream, P);
-  else if (ragged == ROWS) hipLaunchKernelGGL(product_tiles<ROWS>, grid, block, 0, stream, P);
-  else hipLaunchKernelGGL(product_tiles<DEPTH>, grid, block, 0, stream, P);
+  Product P = given;
+  // a dimension of one element has unit stride whatever the tensor says
+  const bool akc = P.a_k == 1 || P.k == 1, amc = P.a_m == 1 || P.m == 1, bkc = P.b_k == 1 || P.k == 1, bnc = P.b_n == 1 || P.n == 1;
+  const long a_pitch = akc ? P.a_m : P.a_k, b_pitch = bkc ? P.b_n : P.b_k;
+  P.slices = 1;
+  if (a_pitch < kFarPitch && b_pitch < kFarPitch && (akc || (amc && bnc))) {
+    const char *force = getenv("THCL_TILE");
+    const int f = force ? atoi(force) : 0;
+    const char *fs = getenv("THCL_SLICES");
+    P.slices = fs ? atoi(fs) : 1;
+    const int groups = P.ragged == DEPTH ? P.groups : 1;
+    if (P.slices > 1) {
+      P.work = (float *)thcl_rt_workspace(rt, (size_t)P.slices * groups * P.m * P.n * sizeof(float));
+      THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
+    }
+    if (f == 1) launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, stream);
+    else if (f == 2) launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, stream);
+    else if (f == 3) launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, stream);
+    else if (f == 4) launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, stream);
+    else launch_split<Tile<256, 128, 4, 2>>(P, akc, bkc && akc, stream);
+    if (P.slices > 1) {
+      check_launch(what);
+      const bool vec = P.n % 4 == 0;
+      const long units = (long)groups * P.m * P.n / (vec ? 4 : 1);
+      const dim3 grid((unsigned)((units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096));
+      if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P, groups);
+      else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P, groups);
+    }
+  } else {
+    unsigned gx = (unsigned)((P.m + kDirectM - 1) / kDirectM), gy = (unsigned)((P.n + kDirectN - 1) / kDirectN);
+    if (P.ragged == ROWS) gx = (unsigned)(P.m / kDirectM + (P.groups < P.m ? P.groups : P.m));
+    THCL_CHECK(gy <= 65535 && P.groups <= 65535, THCL_DIM_WARNING);
+    hipLaunchKernelGGL(product_far, dim3(gx, gy, P.ragged == DEPTH ? P.groups : 1), dim3(256), 0, stream, P);
+  }
   check_launch(what);
   thcl_after_launch(state, rt);
 }
