@@ -237,20 +237,6 @@ constexpr int CHUNKS = KS / 8;
 
 __device__ __forceinline__ unsigned round_pair(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, bf2)); }
 
-__device__ __forceinline__ void split_octet(const float (&x)[8], u4 (&part)[3]) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-    for (int p = 0; p < 3; p++) {
-      const unsigned v = round_pair(a, b);
-      part[p][i] = v;
-      a -= __uint_as_float(v << 16);
-      b -= __uint_as_float(v & 0xffff0000u);
-    }
-  }
-}
-
 // One operand's part of a slab in LDS: [part][chunk of 8 k][line], 16 bytes each, so that a matrix instruction's
 // fragment (32 lines of one chunk in lanes 0-31, of the next in lanes 32-63) is read in one piece.  The lines of a
 // wave are dealt out to its IL tiles in turn (tile t has lines IL i + t), which gives a lane neighbouring columns of
@@ -316,23 +302,36 @@ struct Feed {
       }
     }
   }
-  // LAST: kleft values of k from the slab's first on are the operand's; those behind belong to the next line
-  template <bool LAST>
-  __device__ __forceinline__ void store(char *lds, float (&x)[N][8], int kleft) {
+  __device__ __forceinline__ void store(char *lds, float (&x)[N][8]) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      if (KC && LAST) {
-        const int chunk = (threadIdx.x + TH * i) % CHUNKS;
+    for (int o = 0; o < N; o++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = 8 * chunk + e < kleft ? x[i][e] : 0.f;
+      for (int p = 0; p < 3; p++) {
+        u4 part;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float &a = x[o][2 * i], &b = x[o][2 * i + 1];
+          if (p == 0) least = min(least, min((__float_as_uint(a) << 1) - 1u, (__float_as_uint(b) << 1) - 1u));
+          const unsigned v = round_pair(a, b);
+          part[i] = v;
+          if (p < 2) {
+            a -= __uint_as_float(v << 16);
+            b -= __uint_as_float(v & 0xffff0000u);
+          }
+        }
+        *(u4 *)(lds + to[o] + p * S::PART) = part;
       }
+  }
+  // the last slab: kleft values of k are the operand's; those behind belong to the next line
+  __device__ __forceinline__ void store_last(char *lds, float (&x)[N][8], int kleft) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) least = min(least, (__float_as_uint(x[i][e]) << 1) - 1u);
-      u4 part[3];
-      split_octet(x[i], part);
+    for (int o = 0; o < N; o++)
+      if (KC) {
+        const int chunk = (threadIdx.x + TH * o) % CHUNKS;
 #pragma unroll
-      for (int p = 0; p < 3; p++) *(u4 *)(lds + to[i] + p * S::PART) = part[p];
-    }
+        for (int e = 0; e < 8; e++) x[o][e] = 8 * chunk + e < kleft ? x[o][e] : 0.f;
+      }
+    store(lds, x);
   }
 };
 
@@ -361,7 +360,8 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m
   typedef Feed<T::BN, NT, BKC, T::TH> FB;
   typedef Staged<T::BM, MT> SA;
   typedef Staged<T::BN, NT> SB;
-  __shared__ __attribute__((aligned(16))) char lds[2][T::LDS];
+  // two arrays, so that the compiler knows that the slab being written is not the one being read
+  __shared__ __attribute__((aligned(16))) char lds0[T::LDS], lds1[T::LDS];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
@@ -387,62 +387,78 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m
     for (int j = 0; j < NT; j++) acc[i][j] = f16v{};
 
   const int frag = (lane / 32) * 1, l16 = (lane % 32) * 16;
-  const char *la = &lds[0][0] + frag * SA::CP + (wave / T::WN) * MT * SA::TS + l16;
-  const char *lb = &lds[0][0] + SA::BYTES + frag * SB::CP + (wave % T::WN) * NT * SB::TS + l16;
+  const int la = frag * SA::CP + (wave / T::WN) * MT * SA::TS + l16;
+  const int lb = SA::BYTES + frag * SB::CP + (wave % T::WN) * NT * SB::TS + l16;
 
-  // Slab s is multiplied from one half of LDS while slab s + 1 is split into the other and slab s + 2 is on its way.
-  auto fill = [&](auto last, int set, int half, int s) {
-    fa.template store<decltype(last)::value>(lds[half], xa[set], depth - s * KS);
-    fb.template store<decltype(last)::value>(lds[half] + SA::BYTES, xb[set], depth - s * KS);
-  };
   auto fetch = [&](int set) {
     fa.load(xa[set]);
     fb.load(xb[set]);
   };
+  auto fill = [&](int half, int set) {
+    char *to = half ? lds1 : lds0;
+    fa.store(to, xa[set]);
+    fb.store(to + SA::BYTES, xb[set]);
+  };
+  auto fill_last = [&](int half, int set, int s) {
+    char *to = half ? lds1 : lds0;
+    fa.store_last(to, xa[set], depth - s * KS);
+    fb.store_last(to + SA::BYTES, xb[set], depth - s * KS);
+  };
+  // the products of the slab in one half of LDS
   auto multiply = [&](int half) {
+    const char *from = half ? lds1 : lds0;
     bf8 b[NT][3];
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
-      for (int p = 0; p < 3; p++) b[j][p] = *(const bf8 *)(lb + half * T::LDS + p * SB::PART + j * SB::TS);
+      for (int p = 0; p < 3; p++) b[j][p] = *(const bf8 *)(from + lb + p * SB::PART + j * SB::TS);
+    // tiles two by two down the rows, so that the next product into an accumulator is four instructions away, in an
+    // order in which each instruction shares an operand with the one before it
+    constexpr int PAIR = MT > 1 ? 2 : 1;
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-      bf8 a[3];
+    for (int i0 = 0; i0 < MT; i0 += PAIR) {
+      bf8 a[PAIR][3];
 #pragma unroll
-      for (int p = 0; p < 3; p++) a[p] = *(const bf8 *)(la + half * T::LDS + p * SA::PART + i * SA::TS);
+      for (int i = 0; i < PAIR; i++)
+#pragma unroll
+        for (int p = 0; p < 3; p++) a[i][p] = *(const bf8 *)(from + la + p * SA::PART + (i0 + i) * SA::TS);
       constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
       for (int q = 0; q < 6; q++)
 #pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa[q]], b[j][pb[q]], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < PAIR; i++)
+#pragma unroll
+          for (int jj = 0; jj < NT; jj++) {
+            const int j = i % 2 ? NT - 1 - jj : jj;
+            acc[i0 + i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i][pa[q]], b[j][pb[q]], acc[i0 + i][j], 0, 0, 0);
+          }
     }
   };
+  // Slab s is multiplied from one half of LDS while slab s + 1 is split into the other and slab s + 2 is on its way.
   if (slabs > 0) {
-    const std::false_type whole;
-    const std::true_type last;
     fetch(0);
     fetch(1);
-    fill(last, 0, 0, 0);
+    fill_last(0, 0, 0);
     __syncthreads();
     fetch(0);
     int s = 0;
     // per turn: slab s from half 0, slab s + 1 from half 1; set 1 holds slab s + 1, set 0 slab s + 2
     for (; s + 3 < slabs; s += 2) {
-      fill(whole, 1, 1, s + 1);
+      fill(1, 1);
       fetch(1);
       multiply(0);
       __syncthreads();
-      fill(whole, 0, 0, s + 2);
+      fill(0, 0);
       fetch(0);
       multiply(1);
       __syncthreads();
     }
     // the last one to three
-    if (s + 1 < slabs) fill(last, 1, 1, s + 1);
+    if (s + 1 < slabs) fill_last(1, 1, s + 1);
     multiply(0);
     if (s + 1 < slabs) {
       __syncthreads();
-      if (s + 2 < slabs) fill(last, 0, 0, s + 2);
+      if (s + 2 < slabs) fill_last(0, 0, s + 2);
       multiply(1);
     }
     if (s + 2 < slabs) {
@@ -474,8 +490,9 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m
     }
   // 32 rows at a time through the wave's own part of LDS, so that a lane keeps one column and a wave stores whole rows
   constexpr int COLS = 32 * NT, PER = kWave / COLS > 0 ? kWave / COLS : 1, LANES = COLS < kWave ? COLS : kWave;
-  static_assert(COLS <= kWave && 4 * 32 * COLS * T::WM * T::WN <= 2 * T::LDS, "a wave's rows fit its part of LDS");
-  float *mine = (float *)&lds[0][0] + wave * 32 * COLS;
+  constexpr int WAVES = T::WM * T::WN, HALF = (WAVES + 1) / 2;
+  static_assert(COLS <= kWave && 4 * 32 * COLS * HALF <= T::LDS, "half of the waves' rows fit each half of LDS");
+  float *mine = (float *)(wave < HALF ? lds0 : lds1) + wave % HALF * 32 * COLS;
   const int col = wcol0 + lane % LANES;
   const Column line(P, min(col, P.n - 1));
 #pragma unroll
