@@ -15,6 +15,7 @@
 
 namespace {
 
+typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int kWave = 64;
@@ -44,12 +45,42 @@ struct Column {
   int col;
   float bias;
   __device__ __forceinline__ Column(const Product &P, int c) : col(c), bias(P.bias ? P.bias[c * P.bias_n] : 0.f) {}
+  // rows row, row + step, ... below `rows`; what is read from memory is requested for all of them first
+  template <int N>
+  __device__ __forceinline__ void finish_rows(const Product &P, float *c, int row, int step, int rows, float (&v)[N]) const {
+    float res[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] += bias;
+      res[i] = 0.f;
+    }
+    if (P.residual) {
+#pragma unroll
+      for (int i = 0; i < N; i++) res[i] = P.residual[min(row + step * i, rows - 1) * P.res_m + col];
+    }
+    if (P.preact) {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (row + step * i < rows) P.preact[(row + step * i) * P.pre_m + col] = v[i];
+    }
+    if (P.act != THCL_ACT_NONE) {
+#pragma unroll 1
+      for (int i = 0; i < N; i++) v[0] = activation(P.act, v[0]), rotate(v);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (row + step * i < rows) c[(row + step * i) * P.c_m + col] = v[i] + res[i];
+  }
+  template <int N>
+  static __device__ __forceinline__ void rotate(float (&v)[N]) {
+    const float first = v[0];
+#pragma unroll
+    for (int i = 0; i + 1 < N; i++) v[i] = v[i + 1];
+    v[N - 1] = first;
+  }
   __device__ __forceinline__ void finish(const Product &P, float *c, int row, float v) const {
-    const float res = P.residual ? P.residual[row * P.res_m + col] : 0.f;
-    v += bias;
-    if (P.preact) P.preact[row * P.pre_m + col] = v;
-    v = activation(P.act, v) + res;
-    c[row * P.c_m + col] = v;
+    float one[1] = {v};
+    finish_rows<1>(P, c, row, 1, row + 1, one);
   }
 };
 
@@ -228,7 +259,6 @@ __global__ __launch_bounds__(256) void product_far(Product P) {
 // bf16 values are exact in fp32, and the matrix instructions add them to fp32 accumulators.
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 
@@ -502,17 +532,243 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m
 #pragma unroll
       for (int j = 0; j < NT; j++) mine[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * COLS + NT * (lane % 32) + j] = acc[i][j][r];
     if (col < P.n) {
+      constexpr int FLY = 8;
       float *part = P.slices > 1 ? P.work + (((long)blockIdx.z * gridDim.y + w.group) * P.m) * P.n + col : nullptr;
-      for (int q = lane / LANES; q < 32; q += PER) {
-        const int row = row0 + MT * q + i;
-        const float v = mine[q * COLS + lane % LANES];
-        if (row < w.rows) {
-          if (part) part[(long)row * P.n] = v;
-          else line.finish(P, w.c, row, v);
+#pragma unroll 1
+      for (int q0 = lane / LANES; q0 < 32; q0 += FLY * PER) {
+        float v[FLY];
+#pragma unroll
+        for (int f = 0; f < FLY; f++) v[f] = mine[(q0 + f * PER) * COLS + lane % LANES];
+        const int top = row0 + MT * q0 + i;
+        if (part) {
+#pragma unroll
+          for (int f = 0; f < FLY; f++)
+            if (top + MT * PER * f < w.rows) part[(long)(top + MT * PER * f) * P.n] = v[f];
+        } else {
+          line.finish_rows<FLY>(P, w.c, top, MT * PER, w.rows, v);
         }
       }
     }
   }
+}
+
+// -------------------------------------------------------------- few rows ---
+// Up to 64 rows (a few sequences that generate together, an expert with few tokens) are bound by reading b once.
+// Eight waves share a block's 64 columns, each with its own part of k and no barrier: b streams through registers in
+// steps of 32 k (8 KiB, two steps ahead), and, when it is contiguous along k, through the wave's own corner of LDS,
+// which turns whole 128-byte lines into fragments; the rows of a come from the caches as fragments.  The waves' sums
+// meet in LDS.  Within a step lanes 16 g to 16 g + 15 hold k = 8 g + e of both operands.
+// Up to 32 rows v_mfma_f32_16x16x4_f32 keeps up with memory: 32 cycles for each four k of 16 columns and 16 rows make
+// 256 MT cycles per step and compute unit, against about 800 for its bytes.  Beyond, the operands are split for the
+// bf16 pipes, which takes 192 MT cycles and some 130 (4 + MT) / 4 of vector instructions.
+constexpr int kThinCols = 64, kThinWaves = 8, kThinStep = 32;
+
+template <int MT, bool BKC, bool SPLIT>
+struct ThinStream {
+  static constexpr int PITCH = kThinStep + 4;  // floats: odd number of 16-byte units
+  const char *ab, *bb;
+  long a_left, b_left;
+  unsigned a_off, b_off, least;
+  int a_next, b_next;
+  long b_step;
+  float *turn;
+  typedef float Octet[8];
+
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char *base, long left) {
+    const long l = left < 0 ? 0 : left > 0xffffffffl ? 0xffffffffl : left;
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)l, 0x00020000);
+  }
+  // x[t]: eight k of a's row 16 t + lane % 16; y: contiguous along k, y[2 i + h] is four k (16 h + 4 (lane % 4)...) of
+  // lines of b on their way to LDS, otherwise y[e] is four columns of k = 8 g + e
+  __device__ __forceinline__ void load(Octet (&x)[MT], f4 (&y)[8]) {
+    const __amdgpu_buffer_rsrc_t ra = buffer(ab, a_left), rb = buffer(bb, b_left);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rb, b_off, i * b_next, 2));
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      const f4 lo = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ra, a_off, t * a_next, 0));
+      const f4 hi = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ra, a_off + 16, t * a_next, 0));
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[t][e] = lo[e], x[t][4 + e] = hi[e];
+    }
+    ab += 4 * kThinStep;
+    a_left -= 4 * kThinStep;
+    bb += b_step;
+    b_left -= b_step;
+  }
+  // LAST: kleft values of k from the step's first on are the operands'; what lies behind belongs to the next line
+  template <bool LAST>
+  __device__ __forceinline__ void use(Octet (&x)[MT], f4 (&y)[8], f4 (&acc)[MT][4], int kleft) {
+    const int lane = threadIdx.x % kWave, l16 = lane % 16, g = lane / 16;
+    if (LAST) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) x[t][e] = 8 * g + e < kleft ? x[t][e] : 0.f;
+    }
+    if (BKC) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (LAST)
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[i][e] = 4 * (lane % 8) + e < kleft ? y[i][e] : 0.f;
+        *(f4 *)(turn + (8 * i + lane / 8) * PITCH + 4 * (lane % 8)) = y[i];
+      }
+    }
+    u4 pa[MT][3];
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int t = 0; t < MT; t++) split(x[t], pa[t]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      Octet b;
+      if (BKC) {
+        const f4 lo = *(const f4 *)(turn + (16 * c + l16) * PITCH + 8 * g), hi = *(const f4 *)(turn + (16 * c + l16) * PITCH + 8 * g + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) b[e] = lo[e], b[4 + e] = hi[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) b[e] = y[e][c];
+      }
+      if constexpr (SPLIT) {
+        u4 pb[3];
+        split(b, pb);
+        constexpr int qa[6] = {2, 0, 1, 1, 0, 0}, qb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int q = 0; q < 6; q++)
+#pragma unroll
+          for (int t = 0; t < MT; t++)
+            acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, pa[t][qa[q]]), __builtin_bit_cast(bf8, pb[qb[q]]), acc[t][c], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+          for (int t = 0; t < MT; t++) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][e], b[e], acc[t][c], 0, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void split(Octet x, u4 (&part)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float a = x[2 * i], b = x[2 * i + 1];
+      least = min(least, min((__float_as_uint(a) << 1) - 1u, (__float_as_uint(b) << 1) - 1u));
+#pragma unroll
+      for (int p = 0; p < 3; p++) {
+        const unsigned v = round_pair(a, b);
+        part[p][i] = v;
+        a -= __uint_as_float(v << 16);
+        b -= __uint_as_float(v & 0xffff0000u);
+      }
+    }
+  }
+  // adds steps s0 to s1 of k
+  __device__ __forceinline__ void run(const Product &P, const Work &w, int col0, int s0, int s1, f4 (&acc)[MT][4]) {
+    const int lane = threadIdx.x % kWave, l16 = lane % 16, g = lane / 16;
+    const int rows = min(w.rows - w.row0, 16 * MT), cols = min(P.n - col0, kThinCols);
+    const long k0 = (long)s0 * kThinStep;
+    least = ~0u;
+    ab = (const char *)uniform((long)(P.a + (long)w.row0 * P.a_m + k0));
+    bb = (const char *)uniform((long)(w.b + (long)col0 * P.b_n + k0 * P.b_k));
+    a_left = uniform(4 * ((rows - 1) * P.a_m + P.k - k0));
+    b_left = uniform(4 * ((cols - 1) * P.b_n + (P.k - k0 - 1) * P.b_k + 1));
+    b_step = 4 * kThinStep * P.b_k;
+    a_off = (unsigned)(4 * (l16 * P.a_m + 8 * g));
+    b_off = (unsigned)(BKC ? 4 * ((lane / 8) * P.b_n + 4 * (lane % 8)) : 4 * (8 * g * P.b_k + 4 * l16));
+    b_next = (int)(4 * (BKC ? 8 * P.b_n : P.b_k));
+    a_next = (int)(4 * 16 * P.a_m);
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) acc[t][c] = f4{};
+    if (s0 >= s1) return;
+    Octet x0[MT], x1[MT];
+    f4 y0[8], y1[8];
+    load(x0, y0);
+    load(x1, y1);  // beyond the range it is read for nothing; the buffers end behind the operands
+    int s = s0;
+    for (; s + 2 < s1; s += 2) {
+      use<false>(x0, y0, acc, kThinStep);
+      load(x0, y0);
+      use<false>(x1, y1, acc, kThinStep);
+      load(x1, y1);
+    }
+    use<true>(x0, y0, acc, P.k - s * kThinStep);
+    if (s + 1 < s1) use<true>(x1, y1, acc, P.k - (s + 1) * kThinStep);
+  }
+};
+
+template <int MT, bool BKC, bool SPLIT>
+__global__ __launch_bounds__(64 * kThinWaves, 2) void product_thin(Product P) {
+  constexpr int SUMS = kThinWaves * 16 * kThinCols, TURN = BKC ? kThinWaves * kThinCols * ThinStream<MT, BKC, SPLIT>::PITCH : 0;
+  __shared__ __attribute__((aligned(16))) float lds[SUMS > TURN ? SUMS : TURN];
+  const int wave = uniform((int)threadIdx.x / kWave), lane = threadIdx.x % kWave, l16 = lane % 16, g = lane / 16;
+  Work w;
+  if (!find_work(P, 16 * MT, blockIdx.y, 0, blockIdx.x == 0 && blockIdx.y == 0, w)) return;
+  const int col0 = blockIdx.x * kThinCols, col = col0 + lane;
+  // this wave's steps of k
+  const int all = (P.k + kThinStep - 1) / kThinStep, parts = kThinWaves * P.slices, part = blockIdx.z * kThinWaves + wave;
+  const int s0 = (int)((long)all * part / parts), s1 = (int)((long)all * (part + 1) / parts);
+  f4 acc[MT][4];
+  float sums[MT][2];  // rows 16 t + wave and 16 t + wave + 8 of column `col`
+  // acc[t][c][r] is row 16 t + 4 g + r, column 16 c + l16 (BKC) or 4 l16 + c; the waves' parts are added in wave order
+  auto gather = [&] {
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      __syncthreads();
+      float *mine = lds + wave * 16 * kThinCols;
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) mine[(4 * g + r) * kThinCols + (BKC ? 16 * c + l16 : 4 * l16 + c)] = acc[t][c][r];
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int in = wave + 8 * h;
+        float sum = lds[in * kThinCols + lane];
+#pragma unroll
+        for (int v = 1; v < kThinWaves; v++) sum += lds[(16 * v + in) * kThinCols + lane];
+        sums[t][h] = sum;
+      }
+    }
+  };
+  ThinStream<MT, BKC, SPLIT> stream;
+  stream.turn = lds + wave * kThinCols * ThinStream<MT, BKC, SPLIT>::PITCH;
+  stream.run(P, w, col0, s0, s1, acc);
+  gather();
+  if constexpr (SPLIT) {
+    // what does not split is taken again with fp32 products, as in product_split
+    bool again = false;
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) again |= w.row0 + 16 * t + wave + 8 * h < w.rows && col < P.n && !(fabsf(sums[t][h]) < INFINITY);
+    const bool tiny = __syncthreads_or(stream.least < (17u << 24) - 1u);
+    if (__syncthreads_or(again || tiny)) {
+      float old[MT][2];
+#pragma unroll
+      for (int t = 0; t < MT; t++) old[t][0] = sums[t][0], old[t][1] = sums[t][1];
+      ThinStream<MT, BKC, false> exact;
+      exact.turn = stream.turn;
+      exact.run(P, w, col0, s0, s1, acc);
+      gather();
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (!tiny && fabsf(old[t][h]) < INFINITY) sums[t][h] = old[t][h];
+    }
+  }
+  if (col >= P.n) return;
+#pragma unroll
+  for (int t = 0; t < MT; t++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int row = w.row0 + 16 * t + wave + 8 * h;
+      if (row >= w.rows) continue;
+      if (P.slices > 1) P.work[((long)blockIdx.z * P.m + row) * P.n + col] = sums[t][h];
+      else Column(P, col).finish(P, w.c, row, sums[t][h]);
+    }
 }
 
 // The slices of k of every result, added in order, and the epilogue.
@@ -587,7 +843,16 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
       P.work = (float *)thcl_rt_workspace(rt, (size_t)P.slices * groups * P.m * P.n * sizeof(float));
       THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
     }
-    if (f == 1) launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, stream);
+    if (f >= 5 && akc && P.ragged != DEPTH) {
+      const int mt = f - 4;
+      int tiles_m = (P.m + 16 * mt - 1) / (16 * mt);
+      if (P.ragged == ROWS) tiles_m = P.m / (16 * mt) + (P.groups < P.m ? P.groups : P.m);
+      const dim3 grid((P.n + kThinCols - 1) / kThinCols, tiles_m, P.slices), block(64 * kThinWaves);
+      THCL_CHECK(tiles_m <= 65535, THCL_DIM_WARNING);
+#define GO(MT) if (mt == MT) { if (bkc) hipLaunchKernelGGL((product_thin<MT, true, (MT > 2)>), grid, block, 0, stream, P); else hipLaunchKernelGGL((product_thin<MT, false, (MT > 2)>), grid, block, 0, stream, P); }
+      GO(1) GO(2) GO(3) GO(4)
+#undef GO
+    } else if (f == 1) launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, stream);
     else if (f == 2) launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, stream);
     else if (f == 3) launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, stream);
     else if (f == 4) launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, stream);
