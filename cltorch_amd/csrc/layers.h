@@ -43,6 +43,12 @@ struct Product {
   float *work;
 };
 
+// kind: 0 tiles of 256 x 256, 1 of 128 x 128, 2 of 64 x 128, 3 of 32 x 128, 4 to 7 the kernel for few rows with 16 to
+// 64 of them in a tile
+struct ThclProductPlan {
+  int kind, slices;
+};
+ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus);
 void thcl_product(THClState *state, thcl_rt *rt, const Product &P, const char *what);
 
 // gz = gy act'(z)

@@ -7,7 +7,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -814,64 +813,140 @@ void check_launch(const char *what) {
 }
 }  // namespace
 
+// The kernel for a product, by a small model of the launch in microseconds on 256 compute units, fitted to 25 shapes of
+// 1000 x 64 x 64 to 4096^3 in every tile and 1 to 16 slices of k (the choice was within 13 % of the best of them, in
+// the mean within 1 %):
+//   alone, full   a block's time per slab of 16 k when it has its compute unit to itself, and when `resident` of them
+//                 share one (128 x 128: 0.81 us for one block, 1.33 for two).  The largest tile is the best on a whole
+//                 chip, 234 TFLOP/s against 185 for 128 x 128 and 148 for 64 x 128 at 4096^3, and the worst on part
+//                 of one (1024^3 in 4 slices: 45 us against 29)
+//   start         what a block's first loads and its epilogue cost, in slabs
+//   slices        k is cut when blocks are few: 2048 x 4096 x 4096 in 256 x 256 tiles 449 us, in two slices 323; the
+//                 pass that adds them costs 4.8 us and its bytes
+// Up to 64 rows the kernel for few rows takes part, with what a block of 16 to 64 rows reads per nanosecond (`alone`)
+// and what the chip reaches (1 x 4096 x 16384: 46 us, in tiles 64).
+namespace {
+struct TileCost {
+  int bm, bn, resident;
+  double alone, full, start;
+};
+constexpr TileCost kTiles[4] = {{256, 256, 1, 1.48, 2.09, 6.9}, {128, 128, 2, 0.81, 1.33, 5.5}, {64, 128, 3, 0.60, 1.28, 3.3}, {32, 128, 4, 0.53, 1.34, 1.7}};
+struct ThinCost {
+  double alone, chip;  // bytes per nanosecond
+};
+constexpr ThinCost kThin[4] = {{42., 5800.}, {34., 5500.}, {28., 4800.}, {21.7, 3800.}};
+}  // namespace
+
+ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) {
+  const int groups = P.groups < P.m ? P.groups : P.m;  // that can hold rows
+  const double share = 256. / cus;
+  const double k = P.ragged == DEPTH ? (double)P.k / P.groups : P.k, outputs = (double)P.m * P.n * (P.ragged == DEPTH ? P.groups : 1);
+  ThclProductPlan best{0, 1};
+  double least = INFINITY;
+  auto consider = [&](int kind, int slices, double us) {
+    if (slices > 1) us += 4.8 + 4. * outputs * (2 * slices + 1) / 13800e3;
+    if (us < least) least = us, best = ThclProductPlan{kind, slices};
+  };
+  // row tiles of a ragged product, on the average over where groups end
+  auto row_tiles = [&](int rows) {
+    if (P.ragged != ROWS) return (double)((P.m + rows - 1) / rows);
+    return P.m <= (double)rows * groups ? (double)groups : (double)P.m / rows + 0.5 * groups;
+  };
+  constexpr int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  for (int t = 0; t < 4; t++) {
+    const TileCost &c = kTiles[t];
+    const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
+    for (int s : kSlices) {
+      const double slabs = std::ceil(k / (KS * s));
+      if (s > 1 && (slabs < 4 || s * outputs * 4 > 1e9)) break;
+      const double per = tiles * s * share / 256.;  // blocks to a compute unit
+      auto busy = [&](double n) {
+        if (n <= 1) return c.resident > 1 ? c.alone : c.alone + (c.full - c.alone) * n;
+        return c.alone + (c.full - c.alone) * (n - 1) / (c.resident - 1);
+      };
+      const double whole = per > 1 ? std::ceil(per) : per, turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
+      consider(t, s, 4.1 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (slabs + c.start));
+    }
+  }
+  if (few_rows_fit) {
+    const double rows = P.ragged == ROWS ? (double)P.m / groups : P.m;
+    // a group may hold more than the average: half as much again still fits the tile
+    const int mt = (int)std::ceil(rows * (P.ragged == ROWS ? 1.5 : 1.) / 16);
+    if (mt >= 1 && mt <= 4) {
+      const ThinCost &c = kThin[mt - 1];
+      const double tiles = row_tiles(16 * mt) * ((P.n + kThinCols - 1) / kThinCols), bytes = 4. * P.k * P.n * row_tiles(16 * mt);
+      for (int s : kSlices) {
+        if (s > 1 && (k < 2 * kThinStep * kThinWaves * s || s * outputs * 4 > 1e9)) break;
+        const double rate = std::fmin(tiles * s * c.alone, c.chip / share);
+        consider(4 + mt - 1, s, 4.5 + bytes / rate / 1e3);
+      }
+    }
+  }
+  return best;
+}
+
 template <class T>
-static void launch_split(const Product &P, bool akc, bool bkc, hipStream_t stream) {
+static void launch_split(const Product &P, bool akc, bool bkc, int tiles_m, hipStream_t stream, const char *what) {
   const int tiles_n = (P.n + T::BN - 1) / T::BN;
-  int tiles_m = (P.m + T::BM - 1) / T::BM;
-  if (P.ragged == ROWS) tiles_m = P.m / T::BM + (P.groups < P.m ? P.groups : P.m);
-  THCL_CHECK((long)tiles_m * tiles_n <= INT32_MAX && P.groups <= 65535, THCL_DIM_WARNING);
+  THCL_CHECK((long)tiles_m * tiles_n <= INT32_MAX, THCL_DIM_WARNING);
   const dim3 grid((unsigned)(tiles_m * tiles_n), P.ragged == DEPTH ? P.groups : 1, P.slices), block(T::TH);
   if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true>), grid, block, 0, stream, P, tiles_m, tiles_n);
   else if (akc) hipLaunchKernelGGL((product_split<T, true, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
   else hipLaunchKernelGGL((product_split<T, false, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
+  check_launch(what);
+}
+template <int MT>
+static void launch_thin(const Product &P, bool bkc, int tiles_m, hipStream_t stream, const char *what) {
+  const dim3 grid((P.n + kThinCols - 1) / kThinCols, tiles_m, P.slices), block(64 * kThinWaves);
+  if (bkc) hipLaunchKernelGGL((product_thin<MT, true, (MT > 2)>), grid, block, 0, stream, P);
+  else hipLaunchKernelGGL((product_thin<MT, false, (MT > 2)>), grid, block, 0, stream, P);
+  check_launch(what);
 }
 
 void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const char *what) {
   hipStream_t stream = (hipStream_t)thcl_rt_stream(rt);
   Product P = given;
+  P.slices = 1;
+  THCL_CHECK(P.groups <= 65535, THCL_DIM_WARNING);
+  // blocks by rows: a ragged product may end a tile with each group that holds rows
+  auto row_tiles = [&](int rows) { return P.ragged == ROWS ? P.m / rows + (P.groups < P.m ? P.groups : P.m) : (P.m - 1) / rows + 1; };
   // a dimension of one element has unit stride whatever the tensor says
   const bool akc = P.a_k == 1 || P.k == 1, amc = P.a_m == 1 || P.m == 1, bkc = P.b_k == 1 || P.k == 1, bnc = P.b_n == 1 || P.n == 1;
   const long a_pitch = akc ? P.a_m : P.a_k, b_pitch = bkc ? P.b_n : P.b_k;
-  P.slices = 1;
-  if (a_pitch < kFarPitch && b_pitch < kFarPitch && (akc || (amc && bnc))) {
-    const char *force = getenv("THCL_TILE");
-    const int f = force ? atoi(force) : 0;
-    const char *fs = getenv("THCL_SLICES");
-    P.slices = fs ? atoi(fs) : 1;
-    const int groups = P.ragged == DEPTH ? P.groups : 1;
-    if (P.slices > 1) {
-      P.work = (float *)thcl_rt_workspace(rt, (size_t)P.slices * groups * P.m * P.n * sizeof(float));
-      THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
-    }
-    if (f >= 5 && akc && P.ragged != DEPTH) {
-      const int mt = f - 4;
-      int tiles_m = (P.m + 16 * mt - 1) / (16 * mt);
-      if (P.ragged == ROWS) tiles_m = P.m / (16 * mt) + (P.groups < P.m ? P.groups : P.m);
-      const dim3 grid((P.n + kThinCols - 1) / kThinCols, tiles_m, P.slices), block(64 * kThinWaves);
-      THCL_CHECK(tiles_m <= 65535, THCL_DIM_WARNING);
-#define GO(MT) if (mt == MT) { if (bkc) hipLaunchKernelGGL((product_thin<MT, true, (MT > 2)>), grid, block, 0, stream, P); else hipLaunchKernelGGL((product_thin<MT, false, (MT > 2)>), grid, block, 0, stream, P); }
-      GO(1) GO(2) GO(3) GO(4)
-#undef GO
-    } else if (f == 1) launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, stream);
-    else if (f == 2) launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, stream);
-    else if (f == 3) launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, stream);
-    else if (f == 4) launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, stream);
-    else launch_split<Tile<256, 128, 4, 2>>(P, akc, bkc && akc, stream);
-    if (P.slices > 1) {
-      check_launch(what);
-      const bool vec = P.n % 4 == 0;
-      const long units = (long)groups * P.m * P.n / (vec ? 4 : 1);
-      const dim3 grid((unsigned)((units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096));
-      if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P, groups);
-      else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P, groups);
-    }
-  } else {
-    unsigned gx = (unsigned)((P.m + kDirectM - 1) / kDirectM), gy = (unsigned)((P.n + kDirectN - 1) / kDirectN);
-    if (P.ragged == ROWS) gx = (unsigned)(P.m / kDirectM + (P.groups < P.m ? P.groups : P.m));
-    THCL_CHECK(gy <= 65535 && P.groups <= 65535, THCL_DIM_WARNING);
-    hipLaunchKernelGGL(product_far, dim3(gx, gy, P.ragged == DEPTH ? P.groups : 1), dim3(256), 0, stream, P);
+  if (a_pitch >= kFarPitch || b_pitch >= kFarPitch || !(akc ? bkc || bnc : amc && bnc)) {
+    const unsigned gy = (unsigned)((P.n + kDirectN - 1) / kDirectN);
+    THCL_CHECK(gy <= 65535, THCL_DIM_WARNING);
+    hipLaunchKernelGGL(product_far, dim3((unsigned)row_tiles(kDirectM), gy, P.ragged == DEPTH ? P.groups : 1), dim3(256), 0, stream, P);
+    check_launch(what);
+    thcl_after_launch(state, rt);
+    return;
   }
-  check_launch(what);
+  const bool thin = akc && P.ragged != DEPTH && row_tiles(16) <= 65535;
+  const ThclProductPlan plan = thcl_product_plan(P, thin, thcl_rt_get_props(rt)->compute_units);
+  P.slices = plan.slices;
+  const int groups = P.ragged == DEPTH ? P.groups : 1;
+  if (P.slices > 1) {
+    P.work = (float *)thcl_rt_workspace(rt, (size_t)P.slices * groups * P.m * P.n * sizeof(float));
+    THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
+  }
+  switch (plan.kind) {
+    case 0: launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, row_tiles(256), stream, what); break;
+    case 1: launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, row_tiles(128), stream, what); break;
+    case 2: launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, row_tiles(64), stream, what); break;
+    case 3: launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, row_tiles(32), stream, what); break;
+    case 4: launch_thin<1>(P, bkc, row_tiles(16), stream, what); break;
+    case 5: launch_thin<2>(P, bkc, row_tiles(32), stream, what); break;
+    case 6: launch_thin<3>(P, bkc, row_tiles(48), stream, what); break;
+    default: launch_thin<4>(P, bkc, row_tiles(64), stream, what); break;
+  }
+  if (P.slices > 1) {
+    const bool vec = P.n % 4 == 0;
+    const long units = (long)groups * P.m * P.n / (vec ? 4 : 1);
+    const dim3 grid((unsigned)((units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096));
+    if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P, groups);
+    else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P, groups);
+    check_launch(what);
+  }
   thcl_after_launch(state, rt);
 }
 
