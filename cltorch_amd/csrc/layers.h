@@ -15,6 +15,7 @@ struct NormGradParams {
   const float *gy, *x, *mean, *rstd, *w;
   float *gx, *gw, *gb;
   long rows, width, gy_pitch, x_pitch, gx_pitch, w_step, gw_step, gb_step;
+  double *parts;  // set by thcl_norm_backward: [block][gw, gb][width]
 };
 
 void thcl_norm(THClState *state, thcl_rt *rt, const NormParams &P);
