@@ -39,15 +39,16 @@ struct Product {
   int ragged;          // ThclRagged
   long b_g, c_g;
   unsigned *fault;     // pinned word the host looks at after its next wait
-  // set by thcl_product: k cut into slices, whose partial results lie in work as [slice][group][m][n]
-  int slices;
-  float *work;
+  // set by thcl_product
+  int slices;         // of k, for few rows, whose partial results lie in work as [slice][m][n]
+  int most_sharers;   // blocks to a tile whose slabs of k are shared out
+  float *work;        // [block][2] tiles, or the slices
 };
 
 // kind: 0 tiles of 256 x 256, 1 of 128 x 128, 2 of 64 x 128, 3 of 32 x 128, 4 to 7 the kernel for few rows with 16 to
 // 64 of them in a tile
 struct ThclProductPlan {
-  int kind, slices;
+  int kind, blocks, most_sharers, slices;
 };
 ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus);
 void thcl_product(THClState *state, thcl_rt *rt, const Product &P, const char *what);

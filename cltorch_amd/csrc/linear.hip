@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -87,11 +88,6 @@ struct Column {
 // Where a block's work lies, worked out from the sizes by every wave for itself: lanes take 64 groups at a time and
 // scan them.  Sizes that are no whole numbers, are negative or come to more than `total` rows make the whole call do
 // nothing.
-struct Place {
-  int group;      // -1: no work here
-  int first, count;
-};
-
 __device__ __forceinline__ long wave_scan(long v, int lane) {
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
@@ -101,57 +97,79 @@ __device__ __forceinline__ long wave_scan(long v, int lane) {
   return v;
 }
 
-// rows of all groups together
-__device__ __forceinline__ long count_rows(const float *sizes, int groups, int total, bool &valid) {
-  long rows = 0;
-  valid = true;
-  for (int g0 = 0; g0 < groups && valid; g0 += kWave) {
-    const int g = g0 + threadIdx.x % kWave;
-    const float s = g < groups ? sizes[g] : 0.f;
-    valid = !__any(!(s >= 0.f && s <= (float)total && s == floorf(s)));
-    long n = valid ? (long)s : 0;
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) n += __shfl_xor(n, d, kWave);
-    rows += n;
-    valid = valid && rows <= total;
-  }
-  return rows;
+// A group is made of units: tiles of `unit` rows, the last one not full, and at least `least` of them (unit 0: each group
+// is one).
+__device__ __forceinline__ long units_of(long rows, int unit, int least) {
+  if (!unit) return 1;
+  const long n = (rows + unit - 1) / unit;
+  return n < least ? least : n;
 }
 
-// want: a tile of `tile` rows counted over all groups (tile > 0), or a group (tile == 0)
-__device__ __forceinline__ Place locate(const float *sizes, int groups, int total, int tile, int want, bool &valid) {
+// rows and units of all groups together
+struct Totals {
+  long rows, units;
+  bool valid;
+};
+__device__ __forceinline__ Totals count_groups(const float *sizes, int groups, int total, int unit, int least) {
+  Totals t{0, 0, true};
+  for (int g0 = 0; g0 < groups && t.valid; g0 += kWave) {
+    const int g = g0 + threadIdx.x % kWave;
+    const float s = g < groups ? sizes[g] : 0.f;
+    t.valid = !__any(!(s >= 0.f && s <= (float)total && s == floorf(s)));
+    long n = t.valid ? (long)s : 0, u = t.valid && g < groups ? units_of(n, unit, least) : 0;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+      n += __shfl_xor(n, d, kWave);
+      u += __shfl_xor(u, d, kWave);
+    }
+    t.rows += n;
+    t.units += u;
+    t.valid = t.valid && t.rows <= total;
+  }
+  return t;
+}
+
+// the group of unit `want`, counted over all groups, whose sizes have been found to fit
+struct Place {
+  int group;  // -1: there are fewer units
+  int first, count;
+  long before;  // units of the groups in front
+};
+__device__ __forceinline__ Place locate(const float *sizes, int groups, int unit, int least, long want) {
   const int lane = threadIdx.x % kWave;
-  long rows_before = 0, tiles_before = 0;
-  Place at{-1, 0, 0};
-  valid = true;
+  long rows_before = 0, units_before = 0;
   for (int g0 = 0; g0 < groups; g0 += kWave) {
     const int g = g0 + lane;
-    const float s = g < groups ? sizes[g] : 0.f;
-    const bool ok = s >= 0.f && s <= (float)total && s == floorf(s);
-    if (__any(!ok)) {
-      valid = false;
-      break;
-    }
-    const long n = (long)s, tiles = tile ? (n + tile - 1) / tile : 1;
-    const long rows_in = wave_scan(n, lane), tiles_in = wave_scan(tiles, lane);
-    const bool here = g < groups && want >= tiles_before + tiles_in - tiles && want < tiles_before + tiles_in;
-    const unsigned long long who = __ballot(here);
+    const long n = g < groups ? (long)sizes[g] : 0, units = g < groups ? units_of(n, unit, least) : 0;
+    const long rows_in = wave_scan(n, lane), units_in = wave_scan(units, lane);
+    const unsigned long long who = __ballot(want >= units_before + units_in - units && want < units_before + units_in);
     if (who) {
       const int l = __ffsll((long long)who) - 1;
-      const long first = rows_before + __shfl(rows_in - n, l, kWave), count = __shfl(n, l, kWave);
-      const long skip = tile ? (want - tiles_before - __shfl(tiles_in - tiles, l, kWave)) * tile : 0;
-      at.group = g0 + l;
-      at.first = (int)(first + skip);
-      at.count = (int)(tile ? (count - skip < tile ? count - skip : tile) : count);
+      return Place{g0 + l, (int)(rows_before + __shfl(rows_in - n, l, kWave)), (int)__shfl(n, l, kWave),
+                   units_before + __shfl(units_in - units, l, kWave)};
     }
     rows_before += __shfl(rows_in, kWave - 1, kWave);
-    tiles_before += __shfl(tiles_in, kWave - 1, kWave);
-    if (rows_before > total) {
-      valid = false;
-      break;
-    }
+    units_before += __shfl(units_in, kWave - 1, kWave);
   }
-  return at;
+  return Place{-1, 0, 0, 0};
+}
+
+// group `group`
+__device__ __forceinline__ Place locate_group(const float *sizes, int groups, int unit, int least, int group) {
+  const int lane = threadIdx.x % kWave;
+  long rows = 0, units = 0;
+  for (int g0 = 0; g0 < group; g0 += kWave) {
+    const int g = g0 + lane;
+    const long n = g < group ? (long)sizes[g] : 0;
+    rows += n;
+    units += g < group ? units_of(n, unit, least) : 0;
+  }
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) {
+    rows += __shfl_xor(rows, d, kWave);
+    units += __shfl_xor(units, d, kWave);
+  }
+  return Place{group, (int)rows, (int)sizes[group], units};
 }
 
 // ----------------------------------------------------------------- product ---
@@ -189,43 +207,47 @@ __device__ __forceinline__ long uniform(long v) {
   return (long)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
 }
 
-// What a block works on, the same for every kernel below: rows [row0, rows) and columns [col0, n) of a product over
-// k in [k0, k1).  false: nothing, or sizes that do not fit.
+// a / b of numbers that mostly fit 32 bits, where it takes a tenth of the time
+__device__ __forceinline__ long quotient(long a, long b) {
+  return uniform((a | b) >> 32 ? a / b : (long)((unsigned)a / (unsigned)b));
+}
+
+// A tile's operands and result: rows [row0, rows) of a product over k in [k0, k1).
 struct Work {
   const float *b;
   float *c;
   int row0, rows, k0, k1;
-  int group;
 };
+__device__ __forceinline__ Work whole_work(const Product &P, int tile_rows, int row_tile) { return Work{P.b, P.c, row_tile * tile_rows, P.m, 0, P.k}; }
+__device__ __forceinline__ Work rows_work(const Product &P, int tile_rows, long row_tile) {
+  const Place at = locate(P.sizes, P.groups, tile_rows, 0, row_tile);
+  const int group = uniform(at.group), skip = uniform((int)(row_tile - at.before)) * tile_rows, first = uniform(at.first), count = uniform(at.count);
+  if (group < 0) return Work{P.b, P.c, 0, 0, 0, 0};
+  return Work{P.b + group * P.b_g, P.c, first + skip, first + min(count, skip + tile_rows), 0, P.k};
+}
+__device__ __forceinline__ Work depth_work(const Product &P, int tile_rows, int row_tile, const Place &at) {
+  const int group = uniform(at.group), first = uniform(at.first), count = uniform(at.count);
+  return Work{P.b, P.c + group * P.c_g, row_tile * tile_rows, P.m, first, first + count};
+}
+// false, and the host will hear of it: sizes that do not fit
+__device__ __forceinline__ bool check_groups(const Product &P, int unit, int least, bool first_block, long &units) {
+  const Totals t = count_groups(P.sizes, P.groups, P.ragged == ROWS ? P.m : P.k, unit, least);
+  units = uniform(t.units);
+  if (uniform((int)t.valid)) return true;
+  if (threadIdx.x == 0 && first_block) *P.fault = kFaultGroups;
+  return false;
+}
+// a kernel with a block per row tile (blockIdx.x or y) and, DEPTH, group: false when this one has nothing to do
 __device__ __forceinline__ bool find_work(const Product &P, int tile_rows, int row_tile, int group, bool first_block, Work &w) {
-  w.b = P.b;
-  w.c = P.c;
-  w.row0 = row_tile * tile_rows;
-  w.rows = P.m;
-  w.k0 = 0;
-  w.k1 = P.k;
-  w.group = 0;
-  if (P.ragged == WHOLE) return w.row0 < w.rows;
-  bool valid;
-  const bool by_rows = P.ragged == ROWS;
-  const Place at = locate(P.sizes, P.groups, by_rows ? P.m : P.k, by_rows ? tile_rows : 0, by_rows ? row_tile : group, valid);
-  if (!uniform((int)valid)) {
-    if (threadIdx.x == 0 && first_block) *P.fault = kFaultGroups;
-    return false;
-  }
-  const int group_at = uniform(at.group), first = uniform(at.first), count = uniform(at.count);
-  if (group_at < 0) return false;
-  if (by_rows) {
-    w.row0 = first;
-    w.rows = first + count;
-    w.b += group_at * P.b_g;
+  if (P.ragged == WHOLE) {
+    w = whole_work(P, tile_rows, row_tile);
   } else {
-    w.k0 = first;
-    w.k1 = first + count;
-    w.c += group_at * P.c_g;
-    w.group = group_at;
+    long units;
+    if (!check_groups(P, P.ragged == ROWS ? tile_rows : 0, 0, first_block, units)) return false;
+    if (P.ragged == ROWS) w = rows_work(P, tile_rows, row_tile);
+    else w = depth_work(P, tile_rows, row_tile, locate(P.sizes, P.groups, 0, 0, group));
   }
-  return true;
+  return w.row0 < w.rows;
 }
 
 // Products whose pitches are too long for the tiled kernel's 32-bit offsets.
@@ -368,186 +390,325 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, TH = 64 * WM * WN;
   static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
-  static constexpr int LDS = Staged<BM, MT>::BYTES + Staged<BN, NT>::BYTES;
 };
 
-// logical tile id -> tile coordinates.  Blocks go to the 8 XCDs in turn, and each XCD has its own L2: its blocks get
-// neighbouring ids, and ids walk 8 tiles down the rows before they step along the columns.
-__device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tiles_n, int &tm, int &tn) {
-  const int xcd = id % 8, q = total / 8, r = total % 8;
-  const int lid = xcd * q + min(xcd, r) + id / 8;
-  const int per = 8 * tiles_n, g = lid / per, in = lid % per;
-  const int down = min(tiles_m - 8 * g, 8);
-  tm = 8 * g + in % down;
-  tn = in / down;
+// Blocks go to the 8 XCDs in turn, and each XCD has its own L2: its blocks get neighbouring numbers.
+__device__ __forceinline__ int numbered_by_xcd(int id, int total) { return id % 8 * (total / 8) + min(id % 8, total % 8) + id / 8; }
+// Tile numbers walk 8 tiles down the rows before they step along the columns.
+__device__ __forceinline__ void tile_of(long tile, int tiles_m, int tiles_n, int &tm, int &tn) {
+  const long per = 8l * tiles_n;
+  const int g = (int)quotient(tile, per), in = (int)(tile - g * per), down = min(tiles_m - 8 * g, 8);
+  tn = uniform((int)((unsigned)in / (unsigned)down));
+  tm = uniform(8 * g + in - tn * down);
+}
+// Ragged products: as many blocks as the compute units hold share the slabs of all tiles evenly.  Whole rounds of tiles go to the blocks
+// as they are, and the slabs of the tiles that remain (all of them, when they are fewer than blocks) are cut into equal
+// runs, each a part of one tile or the end of one and the beginning of the next.  The blocks of a tile leave their sums
+// in `work`, two places to a block, and add_parts adds them in the order of k and finishes the tile.  (Added by the
+// block that comes last, in the same launch, they cost more: one compute unit reads some 17 bytes per nanosecond, and
+// 1024^3 in 128 x 128 tiles took 59 us against 29.)
+struct Sharing {
+  int tiles_m, tiles_n, slabs;  // DEPTH: slabs is by group
+  int rounds;
+  long shared, run;             // tiles whose slabs are shared out, in runs of so many
+};
+template <int BM, int BN>
+__device__ __forceinline__ bool share_out(const Product &P, int blocks, bool first_block, Sharing &h) {
+  h.tiles_n = (P.n + BN - 1) / BN;
+  h.tiles_m = (P.m + BM - 1) / BM;
+  h.slabs = (P.k + KS - 1) / KS;
+  h.rounds = 0;
+  long units;
+  if (P.ragged == DEPTH) {
+    if (!check_groups(P, KS, 1, first_block, units)) return false;
+    h.shared = (long)h.tiles_m * h.tiles_n * P.groups;
+    units *= (long)h.tiles_m * h.tiles_n;
+  } else {
+    if (!check_groups(P, BM, 0, first_block, units)) return false;
+    h.tiles_m = (int)units;
+    const long tiles = (long)h.tiles_m * h.tiles_n;
+    h.rounds = (int)quotient(tiles, blocks);
+    h.shared = tiles - (long)h.rounds * blocks;
+    units = h.shared * h.slabs;
+  }
+  const long sharers = min((long)blocks, h.shared * P.most_sharers);
+  h.run = sharers ? max(quotient(units + sharers - 1, sharers), 1l) : 1;
+  return true;
+}
+// where block `block` leaves its sums of the tile that begins at unit0: it has up to two, of the tile that its run ends
+// and of the one that it begins
+__device__ __forceinline__ float *part_of(const Product &P, const Sharing &h, long block, long unit0, int tile_size) {
+  return P.work + (2 * block + (block * h.run >= unit0 ? 0 : 1)) * tile_size;
 }
 
-template <class T, bool AKC, bool BKC>
-__global__ __launch_bounds__(T::TH, 2) void product_split(Product P, int tiles_m, int tiles_n) {
+// RUNS: the ragged products, whose tiles the host cannot count; others have a block to each tile and slice of k, which
+// starts sooner (1000 x 64 x 64: 6.6 us against 8.0) and leaves whole rows of partial results.
+template <class T, bool AKC, bool BKC, bool RUNS>
+__global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
   constexpr int MT = T::MT, NT = T::NT;
   typedef Feed<T::BM, MT, AKC, T::TH> FA;
   typedef Feed<T::BN, NT, BKC, T::TH> FB;
   typedef Staged<T::BM, MT> SA;
   typedef Staged<T::BN, NT> SB;
   // two arrays, so that the compiler knows that the slab being written is not the one being read
-  __shared__ __attribute__((aligned(16))) char lds0[T::LDS], lds1[T::LDS];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  int tm, tn;
-  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
-  Work w;
-  if (!find_work(P, T::BM, tm, blockIdx.y, blockIdx.x == 0 && blockIdx.y == 0, w)) return;
-  const int col0 = tn * T::BN;
-  if (P.slices > 1) {  // this block's slice of k, whole slabs
-    const int per = ((w.k1 - w.k0 + P.slices - 1) / P.slices + KS - 1) / KS * KS;
-    w.k0 = min(w.k0 + (int)blockIdx.z * per, w.k1);
-    w.k1 = min(w.k0 + per, w.k1);
+  __shared__ __attribute__((aligned(16))) char lds0[SA::BYTES + SB::BYTES], lds1[SA::BYTES + SB::BYTES];
+  const int wave = uniform((int)threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int blocks = gridDim.x, me = numbered_by_xcd(blockIdx.x, blocks);
+  Sharing h;
+  long u = 0, u_end = 0;
+  if (RUNS) {
+    if (!share_out<T::BM, T::BN>(P, blocks, blockIdx.x == 0, h)) return;
+    u = uniform(me * h.run);
+    u_end = uniform(P.ragged == DEPTH ? u + h.run : min(u + h.run, h.shared * h.slabs));
+  } else {
+    h = Sharing{(P.m + T::BM - 1) / T::BM, (P.n + T::BN - 1) / T::BN, (P.k + KS - 1) / KS, 1, 0, 1};
   }
+  int round = 0, slabs = h.slabs;
 
-  FA fa;
-  FB fb;
-  fa.begin(P.a, P.a_m, P.a_k, w.row0, w.rows, w.k0, w.k1);
-  fb.begin(w.b, P.b_n, P.b_k, col0, P.n, w.k0, w.k1);
-  const int depth = w.k1 - w.k0, slabs = (depth + KS - 1) / KS;
-  float xa[2][FA::N][8], xb[2][FB::N][8];
-  f16v acc[MT][NT];
+  for (;;) {
+    // the next piece: n slabs from s0 on of a tile that has `slabs` and begins at unit0
+    long tile, unit0 = 0;
+    int s0 = 0, n, tm, tn;
+    Work w;
+    if (RUNS && u < u_end) {
+      if (P.ragged == DEPTH) {
+        const long per_slab = (long)h.tiles_m * h.tiles_n;
+        const Place at = locate(P.sizes, P.groups, KS, 1, quotient(u, per_slab));
+        if (uniform(at.group) < 0) break;  // behind the last group
+        slabs = uniform((int)units_of(at.count, KS, 1));
+        const long in = u - uniform(at.before) * per_slab;
+        tile = quotient(in, slabs);
+        s0 = (int)(in - tile * slabs);
+        tile_of(tile, h.tiles_m, h.tiles_n, tm, tn);
+        w = depth_work(P, T::BM, tm, at);
+      } else {
+        tile = quotient(u, slabs);
+        s0 = (int)(u - tile * slabs);
+      }
+      unit0 = u - s0;
+      n = (int)min((long)(slabs - s0), u_end - u);
+      u += n;
+    } else if (round < h.rounds) {
+      tile = h.shared + (long)round * blocks + me;
+      round++;
+      n = slabs;
+    } else {
+      break;
+    }
+    if (!RUNS) {  // this block's slice of k
+      const int per = (slabs + P.slices - 1) / P.slices;
+      s0 = min((int)blockIdx.z * per, slabs);
+      n = min(per, slabs - s0);
+    }
+    if (!RUNS || P.ragged != DEPTH) {
+      tile_of(tile, h.tiles_m, h.tiles_n, tm, tn);
+      w = RUNS ? rows_work(P, T::BM, tm) : whole_work(P, T::BM, tm);
+    }
+    const int col0 = tn * T::BN;
+    w.k0 += s0 * KS;
+    w.k1 = min(w.k1, w.k0 + n * KS);
+    __syncthreads();  // LDS is free
+    FA fa;
+    FB fb;
+    fa.begin(P.a, P.a_m, P.a_k, w.row0, w.rows, w.k0, w.k1);
+    fb.begin(w.b, P.b_n, P.b_k, col0, P.n, w.k0, w.k1);
+    const int row0 = w.row0 + (wave / T::WN) * 32 * MT, wcol0 = col0 + (wave % T::WN) * 32 * NT;
+    const int depth = w.k1 - w.k0, steps = (depth + KS - 1) / KS;
+    float xa[2][FA::N][8], xb[2][FB::N][8];
+    f16v acc[MT][NT];
 #pragma unroll
-  for (int i = 0; i < MT; i++)
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int j = 0; j < NT; j++) acc[i][j] = f16v{};
+      for (int j = 0; j < NT; j++) acc[i][j] = f16v{};
 
-  const int frag = (lane / 32) * 1, l16 = (lane % 32) * 16;
-  const int la = frag * SA::CP + (wave / T::WN) * MT * SA::TS + l16;
-  const int lb = SA::BYTES + frag * SB::CP + (wave % T::WN) * NT * SB::TS + l16;
+    const int l16 = (lane % 32) * 16;
+    const int la = lane / 32 * SA::CP + (wave / T::WN) * MT * SA::TS + l16;
+    const int lb = SA::BYTES + lane / 32 * SB::CP + (wave % T::WN) * NT * SB::TS + l16;
 
-  auto fetch = [&](int set) {
-    fa.load(xa[set]);
-    fb.load(xb[set]);
-  };
-  auto fill = [&](int half, int set) {
-    char *to = half ? lds1 : lds0;
-    fa.store(to, xa[set]);
-    fb.store(to + SA::BYTES, xb[set]);
-  };
-  auto fill_last = [&](int half, int set, int s) {
-    char *to = half ? lds1 : lds0;
-    fa.store_last(to, xa[set], depth - s * KS);
-    fb.store_last(to + SA::BYTES, xb[set], depth - s * KS);
-  };
-  // the products of the slab in one half of LDS
-  auto multiply = [&](int half) {
-    const char *from = half ? lds1 : lds0;
-    bf8 b[NT][3];
+    auto fetch = [&](int set) {
+      fa.load(xa[set]);
+      fb.load(xb[set]);
+    };
+    auto fill = [&](int half, int set) {
+      char *to = half ? lds1 : lds0;
+      fa.store(to, xa[set]);
+      fb.store(to + SA::BYTES, xb[set]);
+    };
+    auto fill_last = [&](int half, int set, int s) {
+      char *to = half ? lds1 : lds0;
+      fa.store_last(to, xa[set], depth - s * KS);
+      fb.store_last(to + SA::BYTES, xb[set], depth - s * KS);
+    };
+    // the products of the slab in one half of LDS
+    auto multiply = [&](int half) {
+      const char *from = half ? lds1 : lds0;
+      bf8 b[NT][3];
 #pragma unroll
-    for (int j = 0; j < NT; j++)
+      for (int j = 0; j < NT; j++)
 #pragma unroll
-      for (int p = 0; p < 3; p++) b[j][p] = *(const bf8 *)(from + lb + p * SB::PART + j * SB::TS);
-    // tiles two by two down the rows, so that the next product into an accumulator is four instructions away, in an
-    // order in which each instruction shares an operand with the one before it
-    constexpr int PAIR = MT > 1 ? 2 : 1;
+        for (int p = 0; p < 3; p++) b[j][p] = *(const bf8 *)(from + lb + p * SB::PART + j * SB::TS);
+      // tiles two by two down the rows, so that the next product into an accumulator is four instructions away, in an
+      // order in which each instruction shares an operand with the one before it
+      constexpr int PAIR = MT > 1 ? 2 : 1;
 #pragma unroll
-    for (int i0 = 0; i0 < MT; i0 += PAIR) {
-      bf8 a[PAIR][3];
-#pragma unroll
-      for (int i = 0; i < PAIR; i++)
-#pragma unroll
-        for (int p = 0; p < 3; p++) a[i][p] = *(const bf8 *)(from + la + p * SA::PART + (i0 + i) * SA::TS);
-      constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-      for (int q = 0; q < 6; q++)
+      for (int i0 = 0; i0 < MT; i0 += PAIR) {
+        bf8 a[PAIR][3];
 #pragma unroll
         for (int i = 0; i < PAIR; i++)
 #pragma unroll
-          for (int jj = 0; jj < NT; jj++) {
-            const int j = i % 2 ? NT - 1 - jj : jj;
-            acc[i0 + i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i][pa[q]], b[j][pb[q]], acc[i0 + i][j], 0, 0, 0);
-          }
-    }
-  };
-  // Slab s is multiplied from one half of LDS while slab s + 1 is split into the other and slab s + 2 is on its way.
-  if (slabs > 0) {
-    fetch(0);
-    fetch(1);
-    fill_last(0, 0, 0);
-    __syncthreads();
-    fetch(0);
-    int s = 0;
-    // per turn: slab s from half 0, slab s + 1 from half 1; set 1 holds slab s + 1, set 0 slab s + 2
-    for (; s + 3 < slabs; s += 2) {
-      fill(1, 1);
-      fetch(1);
-      multiply(0);
-      __syncthreads();
-      fill(0, 0);
+          for (int p = 0; p < 3; p++) a[i][p] = *(const bf8 *)(from + la + p * SA::PART + (i0 + i) * SA::TS);
+        constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int q = 0; q < 6; q++)
+#pragma unroll
+          for (int i = 0; i < PAIR; i++)
+#pragma unroll
+            for (int jj = 0; jj < NT; jj++) {
+              const int j = i % 2 ? NT - 1 - jj : jj;
+              acc[i0 + i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i][pa[q]], b[j][pb[q]], acc[i0 + i][j], 0, 0, 0);
+            }
+      }
+    };
+    // Slab s is multiplied from one half of LDS while slab s + 1 is split into the other and slab s + 2 is on its way.
+    if (steps > 0) {
       fetch(0);
-      multiply(1);
+      fetch(1);
+      fill_last(0, 0, 0);
       __syncthreads();
-    }
-    // the last one to three
-    if (s + 1 < slabs) fill_last(1, 1, s + 1);
-    multiply(0);
-    if (s + 1 < slabs) {
-      __syncthreads();
-      if (s + 2 < slabs) fill_last(0, 0, s + 2);
-      multiply(1);
-    }
-    if (s + 2 < slabs) {
-      __syncthreads();
+      fetch(0);
+      int s = 0;
+      // per turn: slab s from half 0, slab s + 1 from half 1; set 1 holds slab s + 1, set 0 slab s + 2
+      for (; s + 3 < steps; s += 2) {
+        fill(1, 1);
+        fetch(1);
+        multiply(0);
+        __syncthreads();
+        fill(0, 0);
+        fetch(0);
+        multiply(1);
+        __syncthreads();
+      }
+      // the last one to three
+      if (s + 1 < steps) fill_last(1, 1, s + 1);
       multiply(0);
-    }
-  }
-
-  // What does not split is taken again with fp32 products.  A value that is not finite (or rounds to an infinity) leaves
-  // NaN among its parts, which shows in every result it belongs to; the others stay as they are.  A value below 2^-110
-  // has bits below bf16's smallest, 2^-133; the staging threads have looked out for those.
-  const bool tiny = __syncthreads_or(min(fa.least, fb.least) < (17u << 24) - 1u);  // and LDS is taken for the results below
-  const int row0 = w.row0 + (wave / T::WN) * 32 * MT, wcol0 = col0 + (wave % T::WN) * 32 * NT;
-  if (row0 >= w.rows || wcol0 >= P.n) return;
-  const int colb = wcol0 + NT * (lane % 32);
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      bool again = tiny;
-#pragma unroll
-      for (int r = 0; r < 16; r++)
-        again |= row0 + MT * (8 * (r / 4) + 4 * (lane / 32) + r % 4) + i < w.rows && colb + j < P.n && !(fabsf(acc[i][j][r]) < INFINITY);
-      if (__any(again)) {
-        const f16v v = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0 + i, MT, wcol0 + j, NT, w.k0, w.k1);
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[i][j][r] = tiny || !(fabsf(acc[i][j][r]) < INFINITY) ? v[r] : acc[i][j][r];
+      if (s + 1 < steps) {
+        __syncthreads();
+        if (s + 2 < steps) fill_last(0, 0, s + 2);
+        multiply(1);
+      }
+      if (s + 2 < steps) {
+        __syncthreads();
+        multiply(0);
       }
     }
-  // 32 rows at a time through the wave's own part of LDS, so that a lane keeps one column and a wave stores whole rows
-  constexpr int COLS = 32 * NT, PER = kWave / COLS > 0 ? kWave / COLS : 1, LANES = COLS < kWave ? COLS : kWave;
-  constexpr int WAVES = T::WM * T::WN, HALF = (WAVES + 1) / 2;
-  static_assert(COLS <= kWave && 4 * 32 * COLS * HALF <= T::LDS, "half of the waves' rows fit each half of LDS");
-  float *mine = (float *)(wave < HALF ? lds0 : lds1) + wave % HALF * 32 * COLS;
-  const int col = wcol0 + lane % LANES;
-  const Column line(P, min(col, P.n - 1));
+
+    // What does not split is taken again with fp32 products.  A value that is not finite (or rounds to an infinity) leaves
+    // NaN among its parts, which shows in every result it belongs to; the others stay as they are.  A value below 2^-110
+    // has bits below bf16's smallest, 2^-133; the staging threads have looked out for those.
+    const bool tiny = __syncthreads_or(min(fa.least, fb.least) < (17u << 24) - 1u);  // and LDS is taken for the results below
+    const bool inside = row0 < w.rows && wcol0 < P.n;  // the same for a wave
+    const int colb = wcol0 + NT * (lane % 32);
+    if (inside) {
 #pragma unroll
-  for (int i = 0; i < MT; i++) {
+      for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int r = 0; r < 16; r++)
+        for (int j = 0; j < NT; j++) {
+          bool again = tiny;
 #pragma unroll
-      for (int j = 0; j < NT; j++) mine[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * COLS + NT * (lane % 32) + j] = acc[i][j][r];
-    if (col < P.n) {
-      constexpr int FLY = 8;
-      float *part = P.slices > 1 ? P.work + (((long)blockIdx.z * gridDim.y + w.group) * P.m) * P.n + col : nullptr;
+          for (int r = 0; r < 16; r++)
+            again |= row0 + MT * (8 * (r / 4) + 4 * (lane / 32) + r % 4) + i < w.rows && colb + j < P.n && !(fabsf(acc[i][j][r]) < INFINITY);
+          if (__any(again)) {
+            const f16v v = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0 + i, MT, wcol0 + j, NT, w.k0, w.k1);
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[i][j][r] = tiny || !(fabsf(acc[i][j][r]) < INFINITY) ? v[r] : acc[i][j][r];
+          }
+        }
+    }
+    // 32 rows at a time through the wave's own part of LDS, so that a lane keeps one column and a wave stores whole rows
+    constexpr int COLS = 32 * NT, PER = kWave / COLS > 0 ? kWave / COLS : 1, LANES = COLS < kWave ? COLS : kWave;
+    constexpr int WAVES = T::WM * T::WN, HALF = (WAVES + 1) / 2;
+    static_assert(COLS <= kWave && 4 * 32 * COLS * HALF <= SA::BYTES + SB::BYTES, "half of the waves' rows fit each half of LDS");
+    float *mine = (float *)(wave < HALF ? lds0 : lds1) + wave % HALF * 32 * COLS;
+    const int col = wcol0 + lane % LANES;
+    const Column line(P, min(col, P.n - 1));
+    // partial results: a tile by rows, or, in slices, the whole matrix
+    float *part = nullptr;
+    if (RUNS && n < slabs) part = part_of(P, h, me, unit0, T::BM * T::BN) - (long)w.row0 * T::BN - col0 + col;
+    if (!RUNS && P.slices > 1) part = P.work + (long)blockIdx.z * P.m * P.n + col;
+    const long part_pitch = RUNS ? T::BN : P.n;
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) mine[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * COLS + NT * (lane % 32) + j] = acc[i][j][r];
+        if (col < P.n) {
+          constexpr int FLY = 8;
 #pragma unroll 1
-      for (int q0 = lane / LANES; q0 < 32; q0 += FLY * PER) {
-        float v[FLY];
+          for (int q0 = lane / LANES; q0 < 32; q0 += FLY * PER) {
+            float v[FLY];
 #pragma unroll
-        for (int f = 0; f < FLY; f++) v[f] = mine[(q0 + f * PER) * COLS + lane % LANES];
-        const int top = row0 + MT * q0 + i;
-        if (part) {
+            for (int f = 0; f < FLY; f++) v[f] = mine[(q0 + f * PER) * COLS + lane % LANES];
+            const int top = row0 + MT * q0 + i;
+            if (part) {
 #pragma unroll
-          for (int f = 0; f < FLY; f++)
-            if (top + MT * PER * f < w.rows) part[(long)(top + MT * PER * f) * P.n] = v[f];
-        } else {
-          line.finish_rows<FLY>(P, w.c, top, MT * PER, w.rows, v);
+              for (int f = 0; f < FLY; f++)
+                if (top + MT * PER * f < w.rows) part[(top + MT * PER * f) * part_pitch] = v[f];
+            } else {
+              line.finish_rows<FLY>(P, w.c, top, MT * PER, w.rows, v);
+            }
+          }
         }
       }
     }
+  }
+}
+
+// The parts of the shared tiles, added in the order of k, and the epilogue: a block takes ADD_ROWS rows of a tile
+// (blockIdx.y), a thread four columns.
+constexpr int kAddRows = 16;
+template <int BM, int BN>
+__global__ __launch_bounds__(256) void add_parts(Product P, int blocks) {
+  Sharing h;
+  if (!share_out<BM, BN>(P, blocks, false, h)) return;
+  const long index = blockIdx.x;
+  if (index >= h.shared) return;
+  int tm, tn, slabs = h.slabs;
+  long unit0;
+  Work w;
+  if (P.ragged == DEPTH) {
+    const long tiles = (long)h.tiles_m * h.tiles_n, group = quotient(index, tiles), tile = index - group * tiles;
+    const Place at = locate_group(P.sizes, P.groups, KS, 1, (int)group);
+    slabs = uniform((int)units_of(at.count, KS, 1));
+    unit0 = uniform(at.before) * tiles + tile * slabs;
+    tile_of(tile, h.tiles_m, h.tiles_n, tm, tn);
+    w = depth_work(P, BM, tm, at);
+  } else {
+    unit0 = index * slabs;
+    tile_of(index, h.tiles_m, h.tiles_n, tm, tn);
+    w = rows_work(P, BM, tm);
+  }
+  const long first = quotient(unit0, h.run), last = quotient(unit0 + slabs - 1, h.run);
+  if (first == last) return;  // finished by the block that had all of it
+  constexpr int LANES = BN / 4, ROWS_AT_ONCE = 256 / LANES, N = kAddRows / ROWS_AT_ONCE > 0 ? kAddRows / ROWS_AT_ONCE : 1;
+  const int col = 4 * (threadIdx.x % LANES), row = blockIdx.y * kAddRows + threadIdx.x / LANES;
+  if (w.row0 + row >= w.rows || tn * BN + col >= P.n) return;
+  f4 sum[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) sum[i] = f4{};
+  for (long block = first; block <= last; block++) {
+    const float *p = part_of(P, h, block, unit0, BM * BN) + row * BN + col;
+#pragma unroll
+    for (int i = 0; i < N; i++) sum[i] += *(const f4 *)(p + i * ROWS_AT_ONCE * BN);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (tn * BN + col + e >= P.n) break;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = sum[i][e];
+    Column(P, tn * BN + col + e).finish_rows<N>(P, w.c, w.row0 + row, ROWS_AT_ONCE, w.rows, v);
   }
 }
 
@@ -772,24 +933,22 @@ __global__ __launch_bounds__(64 * kThinWaves, 2) void product_thin(Product P) {
 
 // The slices of k of every result, added in order, and the epilogue.
 template <int VEC>
-__global__ __launch_bounds__(256) void add_slices(Product P, int groups) {
-  int rows = P.m;
-  if (P.ragged != WHOLE) {
-    bool valid;
-    const long total = count_rows(P.sizes, P.groups, P.ragged == ROWS ? P.m : P.k, valid);
-    if (!valid) return;
-    if (P.ragged == ROWS) rows = (int)total;
+__global__ __launch_bounds__(256) void add_slices(Product P) {
+  long rows = P.m;
+  if (P.ragged == ROWS) {
+    const Totals t = count_groups(P.sizes, P.groups, P.m, 0, 0);
+    if (!t.valid) return;
+    rows = t.rows;
   }
-  const long per = (long)P.m * P.n, units = P.n / VEC, all = (long)groups * rows * units;
+  const long per = (long)P.m * P.n, units = P.n / VEC, all = rows * units;
   for (long u = (long)blockIdx.x * 256 + threadIdx.x; u < all; u += (long)gridDim.x * 256) {
-    const long line = u / units;
-    const int col = (int)(u % units) * VEC, row = (int)(line % rows), g = (int)(line / rows);
-    const float *p = P.work + g * per + (long)row * P.n + col;
+    const int col = (int)(u % units) * VEC, row = (int)(u / units);
+    const float *p = P.work + (long)row * P.n + col;
     typedef float V __attribute__((ext_vector_type(VEC)));
     V sum = *(const V *)p;
-    for (int s = 1; s < P.slices; s++) sum += *(const V *)(p + (long)s * groups * per);
+    for (int s = 1; s < P.slices; s++) sum += *(const V *)(p + s * per);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) Column(P, col + e).finish(P, P.c + g * P.c_g, row, sum[e]);
+    for (int e = 0; e < VEC; e++) Column(P, col + e).finish(P, P.c, row, sum[e]);
   }
 }
 
@@ -814,15 +973,13 @@ void check_launch(const char *what) {
 }  // namespace
 
 // The kernel for a product, by a small model of the launch in microseconds on 256 compute units, fitted to 25 shapes of
-// 1000 x 64 x 64 to 4096^3 in every tile and 1 to 16 slices of k (the choice was within 13 % of the best of them, in
-// the mean within 1 %):
+// 1000 x 64 x 64 to 4096^3:
 //   alone, full   a block's time per slab of 16 k when it has its compute unit to itself, and when `resident` of them
 //                 share one (128 x 128: 0.81 us for one block, 1.33 for two).  The largest tile is the best on a whole
 //                 chip, 234 TFLOP/s against 185 for 128 x 128 and 148 for 64 x 128 at 4096^3, and the worst on part
-//                 of one (1024^3 in 4 slices: 45 us against 29)
+//                 of one
 //   start         what a block's first loads and its epilogue cost, in slabs
-//   slices        k is cut when blocks are few: 2048 x 4096 x 4096 in 256 x 256 tiles 449 us, in two slices 323; the
-//                 pass that adds them costs 4.8 us and its bytes
+//   adding        the launch that adds the parts of shared tiles costs 4.8 us and its bytes
 // Up to 64 rows the kernel for few rows takes part, with what a block of 16 to 64 rows reads per nanosecond (`alone`)
 // and what the chip reaches (1 x 4096 x 16384: 46 us, in tiles 64).
 namespace {
@@ -840,45 +997,60 @@ constexpr ThinCost kThin[4] = {{42., 5800.}, {34., 5500.}, {28., 4800.}, {21.7, 
 ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) {
   const int groups = P.groups < P.m ? P.groups : P.m;  // that can hold rows
   const double share = 256. / cus;
-  const double k = P.ragged == DEPTH ? (double)P.k / P.groups : P.k, outputs = (double)P.m * P.n * (P.ragged == DEPTH ? P.groups : 1);
-  ThclProductPlan best{0, 1};
+  const double k = P.ragged == DEPTH ? (double)P.k / P.groups : P.k, outputs = (double)P.m * P.n;
+  ThclProductPlan best{0, 1, 1, 1};
   double least = INFINITY;
-  auto consider = [&](int kind, int slices, double us) {
-    if (slices > 1) us += 4.8 + 4. * outputs * (2 * slices + 1) / 13800e3;
-    if (us < least) least = us, best = ThclProductPlan{kind, slices};
+  auto consider = [&](const ThclProductPlan &plan, double us) {
+    if (us < least) least = us, best = plan;
   };
   // row tiles of a ragged product, on the average over where groups end
   auto row_tiles = [&](int rows) {
     if (P.ragged != ROWS) return (double)((P.m + rows - 1) / rows);
     return P.m <= (double)rows * groups ? (double)groups : (double)P.m / rows + 0.5 * groups;
   };
-  constexpr int kSlices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  const char *ft = getenv("THCL_TILE"), *fs = getenv("THCL_SLICES");
   for (int t = 0; t < 4; t++) {
+    if (ft && atoi(ft) != t + 1) continue;
     const TileCost &c = kTiles[t];
     const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
-    for (int s : kSlices) {
-      const double slabs = std::ceil(k / (KS * s));
-      if (s > 1 && (slabs < 4 || s * outputs * 4 > 1e9)) break;
-      const double per = tiles * s * share / 256.;  // blocks to a compute unit
-      auto busy = [&](double n) {
-        if (n <= 1) return c.resident > 1 ? c.alone : c.alone + (c.full - c.alone) * n;
-        return c.alone + (c.full - c.alone) * (n - 1) / (c.resident - 1);
-      };
-      const double whole = per > 1 ? std::ceil(per) : per, turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
-      consider(t, s, 4.1 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (slabs + c.start));
+    const double slabs = std::fmax(std::ceil(k / KS), 1.);
+    auto busy = [&](double per) {  // a block's time per slab with `per` blocks to a compute unit
+      if (per <= 1) return c.resident > 1 ? c.alone : c.alone + (c.full - c.alone) * per;
+      return c.alone + (c.full - c.alone) * (per - 1) / (c.resident - 1);
+    };
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {  // blocks to a tile
+      if (fs && atoi(fs) != s) continue;
+      if (s > 1 && slabs / s < 4) break;
+      if (P.ragged == WHOLE) {
+        if (s > 1 && s * outputs * 4 > 1e9) break;
+        const double per = tiles * s * share / 256., whole = per > 1 ? std::ceil(per) : per;
+        const double turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
+        double us = 4.1 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (std::ceil(slabs / s) + c.start);
+        if (s > 1) us += 4.8 + 4. * outputs * (2 * s + 1) / 13800e3;
+        consider(ThclProductPlan{t, 1, 1, s}, us);
+      } else {
+        const int blocks = (int)std::fmin((double)cus * c.resident, std::ceil(tiles) * s);
+        const double rounds = P.ragged == DEPTH ? 0. : std::floor(tiles / blocks), shared = tiles - rounds * blocks;
+        const double sharers = std::fmin(blocks, shared * s), run = std::ceil(shared * slabs / sharers);
+        double us = 5.5 + rounds * busy(std::ceil(blocks * share / 256.)) * (slabs + c.start);
+        if (shared > 0) us += busy(std::ceil(sharers * share / 256.)) * (run + c.start);
+        // the parts are written and read, the tiles written
+        if (P.ragged == DEPTH || s > 1) us += 4.8 + 4. * c.bm * c.bn * (2 * sharers + shared) / 13800e3;
+        consider(ThclProductPlan{t, blocks, s, 1}, us);
+      }
     }
   }
-  if (few_rows_fit) {
+  if (few_rows_fit && !ft) {
     const double rows = P.ragged == ROWS ? (double)P.m / groups : P.m;
     // a group may hold more than the average: half as much again still fits the tile
     const int mt = (int)std::ceil(rows * (P.ragged == ROWS ? 1.5 : 1.) / 16);
     if (mt >= 1 && mt <= 4) {
       const ThinCost &c = kThin[mt - 1];
       const double tiles = row_tiles(16 * mt) * ((P.n + kThinCols - 1) / kThinCols), bytes = 4. * P.k * P.n * row_tiles(16 * mt);
-      for (int s : kSlices) {
+      for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (s > 1 && (k < 2 * kThinStep * kThinWaves * s || s * outputs * 4 > 1e9)) break;
         const double rate = std::fmin(tiles * s * c.alone, c.chip / share);
-        consider(4 + mt - 1, s, 4.5 + bytes / rate / 1e3);
+        consider(ThclProductPlan{4 + mt - 1, 1, 1, s}, 4.5 + bytes / rate / 1e3 + (s > 1 ? 4.8 + 4. * outputs * (2 * s + 1) / 13800e3 : 0.));
       }
     }
   }
@@ -886,13 +1058,27 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
 }
 
 template <class T>
-static void launch_split(const Product &P, bool akc, bool bkc, int tiles_m, hipStream_t stream, const char *what) {
-  const int tiles_n = (P.n + T::BN - 1) / T::BN;
-  THCL_CHECK((long)tiles_m * tiles_n <= INT32_MAX, THCL_DIM_WARNING);
-  const dim3 grid((unsigned)(tiles_m * tiles_n), P.ragged == DEPTH ? P.groups : 1, P.slices), block(T::TH);
-  if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true>), grid, block, 0, stream, P, tiles_m, tiles_n);
-  else if (akc) hipLaunchKernelGGL((product_split<T, true, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
-  else hipLaunchKernelGGL((product_split<T, false, false>), grid, block, 0, stream, P, tiles_m, tiles_n);
+static void launch_split(const Product &P, bool akc, bool bkc, int blocks, hipStream_t stream, const char *what) {
+  const dim3 block(T::TH);
+  const long tiles_m = (P.m - 1) / T::BM + 1, tiles_n = (P.n - 1) / T::BN + 1;
+  THCL_CHECK(tiles_m * tiles_n <= INT32_MAX, THCL_DIM_WARNING);
+  if (P.ragged == WHOLE) {
+    const dim3 grid((unsigned)(tiles_m * tiles_n), 1, P.slices);
+    if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true, false>), grid, block, 0, stream, P);
+    else if (akc) hipLaunchKernelGGL((product_split<T, true, false, false>), grid, block, 0, stream, P);
+    else hipLaunchKernelGGL((product_split<T, false, false, false>), grid, block, 0, stream, P);
+    check_launch(what);
+    return;
+  }
+  if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true, true>), dim3(blocks), block, 0, stream, P);
+  else if (akc) hipLaunchKernelGGL((product_split<T, true, false, true>), dim3(blocks), block, 0, stream, P);
+  else hipLaunchKernelGGL((product_split<T, false, false, true>), dim3(blocks), block, 0, stream, P);
+  check_launch(what);
+  if (P.ragged == ROWS && P.most_sharers < 2) return;  // runs of whole tiles
+  // the tiles that may have been shared
+  const long shared = P.ragged == DEPTH ? tiles_m * tiles_n * P.groups : blocks;
+  THCL_CHECK(shared <= INT32_MAX, THCL_DIM_WARNING);
+  hipLaunchKernelGGL((add_parts<T::BM, T::BN>), dim3((unsigned)shared, T::BM / kAddRows), dim3(256), 0, stream, P, blocks);
   check_launch(what);
 }
 template <int MT>
@@ -923,17 +1109,20 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
   }
   const bool thin = akc && P.ragged != DEPTH && row_tiles(16) <= 65535;
   const ThclProductPlan plan = thcl_product_plan(P, thin, thcl_rt_get_props(rt)->compute_units);
+  P.most_sharers = plan.most_sharers;
   P.slices = plan.slices;
-  const int groups = P.ragged == DEPTH ? P.groups : 1;
-  if (P.slices > 1) {
-    P.work = (float *)thcl_rt_workspace(rt, (size_t)P.slices * groups * P.m * P.n * sizeof(float));
+  size_t floats = 0;
+  if (P.slices > 1) floats = (size_t)P.slices * P.m * P.n;
+  else if (plan.kind < 4 && P.ragged != WHOLE) floats = 2ul * plan.blocks * kTiles[plan.kind].bm * kTiles[plan.kind].bn;
+  if (floats) {
+    P.work = (float *)thcl_rt_workspace(rt, floats * sizeof(float));
     THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
   }
   switch (plan.kind) {
-    case 0: launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, row_tiles(256), stream, what); break;
-    case 1: launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, row_tiles(128), stream, what); break;
-    case 2: launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, row_tiles(64), stream, what); break;
-    case 3: launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, row_tiles(32), stream, what); break;
+    case 0: launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 1: launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 2: launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 3: launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
     case 4: launch_thin<1>(P, bkc, row_tiles(16), stream, what); break;
     case 5: launch_thin<2>(P, bkc, row_tiles(32), stream, what); break;
     case 6: launch_thin<3>(P, bkc, row_tiles(48), stream, what); break;
@@ -941,10 +1130,10 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
   }
   if (P.slices > 1) {
     const bool vec = P.n % 4 == 0;
-    const long units = (long)groups * P.m * P.n / (vec ? 4 : 1);
+    const long units = (long)P.m * P.n / (vec ? 4 : 1);
     const dim3 grid((unsigned)((units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096));
-    if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P, groups);
-    else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P, groups);
+    if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P);
+    else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P);
     check_launch(what);
   }
   thcl_after_launch(state, rt);
