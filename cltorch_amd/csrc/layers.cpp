@@ -266,14 +266,25 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
   ThclTemp gz(state, nullptr);
   RowsIn gy(state, gradOutput);
   Rows g = gy;
-  if (slope) {
-    RowsIn z(state, preact);
-    gz.t = THClTensor_newv2(state, THClTensor_getDevice(state, gradOutput));
-    Shape s = shape2(M, N);
-    s.give(state, gz.t);
-    thcl_as_rows(gz.t, g);
-    thcl_activation_slope(state, thcl_ctx(state, THClTensor_getDevice(state, src)),
-                          SlopeParams{gy.p, z.p, g.p, gy.pitch, z.pitch, g.pitch, M, N, activation});
+  const bool products = gradInput || gradWeight;
+  if ((slope && products) || gradBias) {
+    std::optional<RowsIn> z;
+    SlopeParams S;
+    memset(&S, 0, sizeof(S));
+    S.gy = gy.p, S.gy_pitch = gy.pitch;
+    S.rows = M, S.width = N, S.act = activation;
+    if (slope) {
+      z.emplace(state, preact);
+      S.z = z->p, S.z_pitch = z->pitch;
+    }
+    if (slope && products) {
+      gz.t = THClTensor_newv2(state, THClTensor_getDevice(state, gradOutput));
+      shape2(M, N).give(state, gz.t);
+      thcl_as_rows(gz.t, g);
+      S.gz = g.p, S.gz_pitch = g.pitch;
+    }
+    if (gradBias) S.gb = thcl_dptr(gradBias), S.gb_step = gradBias->stride[0];
+    thcl_slope(state, thcl_ctx(state, THClTensor_getDevice(state, src)), S);
   }
   Product P;
   memset(&P, 0, sizeof(P));
@@ -296,15 +307,6 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
     P.m = (int)N, P.n = (int)K, P.k = (int)M;
     thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linearBackward");
     gw.finish();
-  }
-  if (gradBias) {
-    // the library's own column sum
-    THClTensor *from = slope ? gz.t : gy.copy.t ? gy.copy.t : gradOutput;
-    ThclTemp rows(state, THClTensor_newWithStorage2d(state, THClTensor_getDevice(state, src), from->storage, from->storageOffset, M, g.pitch, N, 1));
-    ThclTemp sum(state, THClTensor_newv2(state, THClTensor_getDevice(state, src)));
-    THClTensor_sum(state, sum.t, rows.t, 0);
-    ThclTemp row(state, THClTensor_newSelect(state, sum.t, 0, 0));
-    THClTensor_copy(state, gradBias, row.t);
   }
   THCL_GUARD_END()
 }

@@ -53,12 +53,15 @@ struct ThclProductPlan {
 ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus);
 void thcl_product(THClState *state, thcl_rt *rt, const Product &P, const char *what);
 
-// gz = gy act'(z)
+// gz = gy act'(z) and the sums of its columns; gz or gb is NULL when it is not wanted
 struct SlopeParams {
   const float *gy, *z;
-  float *gz;
-  long gy_pitch, z_pitch, gz_pitch;
+  float *gz, *gb;
+  long gy_pitch, z_pitch, gz_pitch, gb_step;
   long rows, width;
   int act;
+  // set by thcl_slope: rows to a part of the sums, and those
+  long run;
+  double *parts;
 };
-void thcl_activation_slope(THClState *state, thcl_rt *rt, const SlopeParams &P);
+void thcl_slope(THClState *state, thcl_rt *rt, const SlopeParams &P);

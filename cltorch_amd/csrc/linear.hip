@@ -23,21 +23,59 @@ constexpr int kWave = 64;
 constexpr unsigned kFaultGroups = 3u;
 
 // ------------------------------------------------------------- activations ---
-__device__ __forceinline__ float activation(int act, float z) {
-  if (act == THCL_ACT_RELU) return z < 0.f ? 0.f : z;
-  // z times the normal distribution's mass below z; erfc keeps the digits of the lower tail
-  if (act == THCL_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-  if (act == THCL_ACT_SILU) return z / (1.f + expf(-z));
-  return z;
+// Written out here because the mathematical library's erfc and exp, with their branches, took as long as the products of
+// a layer 1024 wide (1531 x 1027 x 2053 with gelu: 87 us, without 61).
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.9259629911e-8f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float reciprocal(float d) {  // a step of Newton's method from the chip's estimate
+  const float r = __builtin_amdgcn_rcpf(d);
+  return fmaf(r, fmaf(-d, r, 1.f), r);
 }
-__device__ __forceinline__ float activation_slope(int act, float z) {
-  if (act == THCL_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == THCL_ACT_GELU) return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * erfcf(-0.70710678118654752f * z));
-  if (act == THCL_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-z));
-    return s * fmaf(z, 1.f - s, 1.f);
-  }
-  return 1.f;
+// 2^(h + l), l small against a rounding of h
+__device__ __forceinline__ float exp2_sum(float h, float l) {
+  const float e = __builtin_amdgcn_exp2f(h);
+  return fmaf(e, l * kLn2, e);
+}
+__device__ __forceinline__ float sigmoid(float z) {
+  const float h = -z * kLog2e, l = fmaf(-z, kLog2e, -h) - z * kLog2eRest;
+  // up to 2^120: beyond, one more than it is no more than it, and its reciprocal is nothing beside any z
+  return reciprocal(1.f + exp2_sum(fminf(h, 120.f), h < 120.f ? l : 0.f));
+}
+// The part of the normal distribution beyond |z| on both sides, erfc(x) with x = |z| / sqrt(2), and exp(-x^2).  With
+// t = 3 / (3 + x), erfc(x) exp(x^2) / t is a polynomial of degree 9 in t to 8e-9 of its value, fitted to erfcx over x up
+// to 14.2; x^2 is taken in two floats, so the tail keeps its digits.
+__device__ __forceinline__ float two_tails(float a, float &gauss) {
+  const float x = a * 0.70710678118654752f, t = 3.f * reciprocal(3.f + x);
+  float p = 0.0516761677250975f;
+  p = fmaf(p, t, -0.2703980393678259f);
+  p = fmaf(p, t, 0.48504998923388043f);
+  p = fmaf(p, t, -0.37421562508419004f);
+  p = fmaf(p, t, 0.34832457015401336f);
+  p = fmaf(p, t, 0.027439353391789156f);
+  p = fmaf(p, t, 0.18207983347981813f);
+  p = fmaf(p, t, 0.17356429719995523f);
+  p = fmaf(p, t, 0.18843063685731984f);
+  p = fmaf(p, t, 0.18804880854297287f);
+  const float q = x * x, h = -q * kLog2e;
+  gauss = exp2_sum(h, (fmaf(-q, kLog2e, -h) - q * kLog2eRest) - fmaf(x, x, -q) * kLog2e);
+  return t * p * gauss;
+}
+// z times the normal distribution's mass below z: 0 for minus infinity
+__device__ __forceinline__ float gelu(float z) {
+  float gauss;
+  const float a = fminf(fabsf(z), 20.f);  // whose tails are nothing
+  const float tails = 0.5f * a * two_tails(a, gauss);
+  return z != z ? z : fmaxf(z, 0.f) - tails;
+}
+__device__ __forceinline__ float gelu_slope(float z) {
+  float gauss;
+  const float half = 0.5f * two_tails(fminf(fabsf(z), 20.f), gauss);
+  return z != z ? z : fmaf(fmaxf(fminf(z, 20.f), -20.f) * 0.3989422804014327f, gauss, z > 0.f ? 1.f - half : half);
+}
+__device__ __forceinline__ float silu(float z) { return z < -104.f ? -0.f : z * sigmoid(z); }
+__device__ __forceinline__ float silu_slope(float z) {
+  const float s = sigmoid(z);
+  return fabsf(z) > 104.f ? (z > 0.f ? 1.f : 0.f) : s * fmaf(z, 1.f - s, 1.f);
 }
 
 // the epilogue of one column of the result
@@ -63,20 +101,19 @@ struct Column {
       for (int i = 0; i < N; i++)
         if (row + step * i < rows) P.preact[(row + step * i) * P.pre_m + col] = v[i];
     }
-    if (P.act != THCL_ACT_NONE) {
-#pragma unroll 1
-      for (int i = 0; i < N; i++) v[0] = activation(P.act, v[0]), rotate(v);
+    if (P.act == THCL_ACT_RELU) {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+    } else if (P.act == THCL_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
+    } else if (P.act == THCL_ACT_SILU) {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = silu(v[i]);
     }
 #pragma unroll
     for (int i = 0; i < N; i++)
       if (row + step * i < rows) c[(row + step * i) * P.c_m + col] = v[i] + res[i];
-  }
-  template <int N>
-  static __device__ __forceinline__ void rotate(float (&v)[N]) {
-    const float first = v[0];
-#pragma unroll
-    for (int i = 0; i + 1 < N; i++) v[i] = v[i + 1];
-    v[N - 1] = first;
   }
   __device__ __forceinline__ void finish(const Product &P, float *c, int row, float v) const {
     float one[1] = {v};
@@ -665,8 +702,8 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
   }
 }
 
-// The parts of the shared tiles, added in the order of k, and the epilogue: a block takes ADD_ROWS rows of a tile
-// (blockIdx.y), a thread four columns.
+// The parts of the shared tiles, added in the order of k, and the epilogue: a block takes 16 rows of a tile
+// (blockIdx.y), a thread a column.
 constexpr int kAddRows = 16;
 template <int BM, int BN>
 __global__ __launch_bounds__(256) void add_parts(Product P, int blocks) {
@@ -691,25 +728,18 @@ __global__ __launch_bounds__(256) void add_parts(Product P, int blocks) {
   }
   const long first = quotient(unit0, h.run), last = quotient(unit0 + slabs - 1, h.run);
   if (first == last) return;  // finished by the block that had all of it
-  constexpr int LANES = BN / 4, ROWS_AT_ONCE = 256 / LANES, N = kAddRows / ROWS_AT_ONCE > 0 ? kAddRows / ROWS_AT_ONCE : 1;
-  const int col = 4 * (threadIdx.x % LANES), row = blockIdx.y * kAddRows + threadIdx.x / LANES;
+  constexpr int ROWS_AT_ONCE = 256 / BN, N = kAddRows / ROWS_AT_ONCE;
+  const int col = threadIdx.x % BN, row = blockIdx.y * kAddRows + threadIdx.x / BN;
   if (w.row0 + row >= w.rows || tn * BN + col >= P.n) return;
-  f4 sum[N];
+  float sum[N];
 #pragma unroll
-  for (int i = 0; i < N; i++) sum[i] = f4{};
+  for (int i = 0; i < N; i++) sum[i] = 0.f;
   for (long block = first; block <= last; block++) {
     const float *p = part_of(P, h, block, unit0, BM * BN) + row * BN + col;
 #pragma unroll
-    for (int i = 0; i < N; i++) sum[i] += *(const f4 *)(p + i * ROWS_AT_ONCE * BN);
+    for (int i = 0; i < N; i++) sum[i] += p[i * ROWS_AT_ONCE * BN];
   }
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    if (tn * BN + col + e >= P.n) break;
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = sum[i][e];
-    Column(P, tn * BN + col + e).finish_rows<N>(P, w.c, w.row0 + row, ROWS_AT_ONCE, w.rows, v);
-  }
+  Column(P, tn * BN + col).finish_rows<N>(P, w.c, w.row0 + row, ROWS_AT_ONCE, w.rows, sum);
 }
 
 // -------------------------------------------------------------- few rows ---
@@ -931,37 +961,72 @@ __global__ __launch_bounds__(64 * kThinWaves, 2) void product_thin(Product P) {
     }
 }
 
-// The slices of k of every result, added in order, and the epilogue.
-template <int VEC>
+// The slices of k of every result, added in order, and the epilogue: a block takes 256 columns of 8 rows, walking down.
+constexpr int kSliceRows = 8;
 __global__ __launch_bounds__(256) void add_slices(Product P) {
-  long rows = P.m;
+  int rows = P.m;
   if (P.ragged == ROWS) {
     const Totals t = count_groups(P.sizes, P.groups, P.m, 0, 0);
     if (!t.valid) return;
-    rows = t.rows;
+    rows = (int)t.rows;
   }
-  const long per = (long)P.m * P.n, units = P.n / VEC, all = rows * units;
-  for (long u = (long)blockIdx.x * 256 + threadIdx.x; u < all; u += (long)gridDim.x * 256) {
-    const int col = (int)(u % units) * VEC, row = (int)(u / units);
-    const float *p = P.work + (long)row * P.n + col;
-    typedef float V __attribute__((ext_vector_type(VEC)));
-    V sum = *(const V *)p;
-    for (int s = 1; s < P.slices; s++) sum += *(const V *)(p + s * per);
-#pragma unroll
-    for (int e = 0; e < VEC; e++) Column(P, col + e).finish(P, P.c, row, sum[e]);
-  }
-}
-
-// gz = gy act'(z)
-__global__ __launch_bounds__(256) void slope_rows(SlopeParams P) {
   const int col = blockIdx.x * 256 + threadIdx.x;
-  const long row = blockIdx.y;
-  if (col >= P.width) return;
-  const float z = P.z[row * P.z_pitch + col], g = P.gy[row * P.gy_pitch + col];
-  // the flat half of relu passes nothing on, whatever comes back
-  P.gz[row * P.gz_pitch + col] = P.act == THCL_ACT_RELU ? (z > 0.f ? g : 0.f) : g * activation_slope(P.act, z);
+  if (col >= P.n) return;
+  const Column line(P, col);
+  const long per = (long)P.m * P.n;
+  for (long row = (long)blockIdx.y * kSliceRows; row < rows; row += (long)gridDim.y * kSliceRows) {
+    float sum[kSliceRows];
+#pragma unroll
+    for (int i = 0; i < kSliceRows; i++) sum[i] = 0.f;
+    for (int s = 0; s < P.slices; s++) {
+      const float *p = P.work + s * per + col;
+#pragma unroll
+      for (int i = 0; i < kSliceRows; i++) sum[i] += p[min(row + i, (long)rows - 1) * P.n];
+    }
+    line.finish_rows<kSliceRows>(P, P.c, (int)row, 1, rows, sum);
+  }
 }
 
+// gz = gy act'(z), and the sums of its columns: a block takes 256 columns of a run of rows and leaves its part of the
+// sums, in fp64 like the library's other sums.
+template <int ACT, bool WRITE, bool SUM>
+__global__ __launch_bounds__(256) void slope_columns(SlopeParams P) {
+  const long col = (long)blockIdx.x * 256 + threadIdx.x;
+  if (col >= P.width) return;
+  const long r1 = min((long)(blockIdx.y + 1) * P.run, P.rows);
+  double sum = 0.0;
+#pragma unroll 4
+  for (long r = (long)blockIdx.y * P.run; r < r1; r++) {
+    float g = P.gy[r * P.gy_pitch + col];
+    if (ACT != THCL_ACT_NONE) {
+      const float z = P.z[r * P.z_pitch + col];
+      // the flat half of relu passes nothing on, whatever comes back
+      if (ACT == THCL_ACT_RELU) g = z > 0.f ? g : 0.f;
+      if (ACT == THCL_ACT_GELU) g *= gelu_slope(z);
+      if (ACT == THCL_ACT_SILU) g *= silu_slope(z);
+    }
+    if (WRITE) P.gz[r * P.gz_pitch + col] = g;
+    if (SUM) sum += (double)g;
+  }
+  if (SUM) P.parts[blockIdx.y * P.width + col] = sum;
+}
+// 16 columns to a block, each by 16 threads that take a run of the parts
+__global__ __launch_bounds__(256) void slope_fold(SlopeParams P, int parts) {
+  __shared__ double sums[16][16];
+  const int lane = threadIdx.x % 16, run = threadIdx.x / 16;
+  const long col = (long)blockIdx.x * 16 + lane;
+  const int p0 = (int)((long)parts * run / 16), p1 = (int)((long)parts * (run + 1) / 16);
+  double s = 0.0;
+  if (col < P.width)
+#pragma unroll 8
+    for (int p = p0; p < p1; p++) s += P.parts[p * P.width + col];
+  sums[run][lane] = s;
+  __syncthreads();
+  if (run != 0 || col >= P.width) return;
+#pragma unroll
+  for (int i = 1; i < 16; i++) s += sums[i][lane];
+  P.gb[col * P.gb_step] = (float)s;
+}
 
 // an operand's pitch from which a tile's lines no longer fit 32-bit byte offsets
 constexpr long kFarPitch = 1l << 21;
@@ -1129,22 +1194,38 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
     default: launch_thin<4>(P, bkc, row_tiles(64), stream, what); break;
   }
   if (P.slices > 1) {
-    const bool vec = P.n % 4 == 0;
-    const long units = (long)P.m * P.n / (vec ? 4 : 1);
-    const dim3 grid((unsigned)((units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096));
-    if (vec) hipLaunchKernelGGL(add_slices<4>, grid, dim3(256), 0, stream, P);
-    else hipLaunchKernelGGL(add_slices<1>, grid, dim3(256), 0, stream, P);
+    const int down = (P.m - 1) / kSliceRows + 1;
+    hipLaunchKernelGGL(add_slices, dim3((unsigned)((P.n - 1) / 256 + 1), (unsigned)(down < 65535 ? down : 65535)), dim3(256), 0, stream, P);
     check_launch(what);
   }
   thcl_after_launch(state, rt);
 }
 
-void thcl_activation_slope(THClState *state, thcl_rt *rt, const SlopeParams &P) {
-  for (long r0 = 0; r0 < P.rows; r0 += 65535) {
-    SlopeParams Q = P;
-    Q.gy += r0 * P.gy_pitch, Q.z += r0 * P.z_pitch, Q.gz += r0 * P.gz_pitch;
-    Q.rows = P.rows - r0 < 65535 ? P.rows - r0 : 65535;
-    hipLaunchKernelGGL(slope_rows, dim3((unsigned)((P.width + 255) / 256), (unsigned)Q.rows), dim3(256), 0, (hipStream_t)thcl_rt_stream(rt), Q);
+void thcl_slope(THClState *state, thcl_rt *rt, const SlopeParams &given) {
+  hipStream_t stream = (hipStream_t)thcl_rt_stream(rt);
+  SlopeParams P = given;
+  // four blocks to a compute unit, and at least 8 rows to a part
+  const long across = (P.width - 1) / 256 + 1, want = 4l * thcl_rt_get_props(rt)->compute_units / across + 1;
+  P.run = (P.rows - 1) / want + 1;
+  if (P.run < 8) P.run = 8;
+  const long parts = (P.rows - 1) / P.run + 1;
+  THCL_CHECK(across <= INT32_MAX && parts <= 65535, THCL_DIM_WARNING);
+  if (P.gb) {
+    P.parts = (double *)thcl_rt_workspace(rt, (size_t)parts * P.width * sizeof(double));
+    THCL_CHECK(P.parts != nullptr, "linearBackward workspace: %s", thcl_rt_error());
+  }
+  const dim3 grid((unsigned)across, (unsigned)parts), block(256);
+#define GO(ACT)                                                                                                  \
+  if (P.act == ACT) {                                                                                            \
+    if (P.gz && P.gb) hipLaunchKernelGGL((slope_columns<ACT, true, true>), grid, block, 0, stream, P);           \
+    else if (P.gz) hipLaunchKernelGGL((slope_columns<ACT, true, false>), grid, block, 0, stream, P);             \
+    else hipLaunchKernelGGL((slope_columns<ACT, false, true>), grid, block, 0, stream, P);                       \
+  }
+  GO(THCL_ACT_NONE) GO(THCL_ACT_RELU) GO(THCL_ACT_GELU) GO(THCL_ACT_SILU)
+#undef GO
+  check_launch("linearBackward");
+  if (P.gb) {
+    hipLaunchKernelGGL(slope_fold, dim3((unsigned)((P.width - 1) / 16 + 1)), dim3(256), 0, stream, P, (int)parts);
     check_launch("linearBackward");
   }
   thcl_after_launch(state, rt);
