@@ -134,26 +134,29 @@ __device__ __forceinline__ long wave_scan(long v, int lane) {
   return v;
 }
 
-// A group is made of units: tiles of `unit` rows, the last one not full, and at least `least` of them (unit 0: each group
-// is one).
-__device__ __forceinline__ long units_of(long rows, int unit, int least) {
-  if (!unit) return 1;
-  const long n = (rows + unit - 1) / unit;
-  return n < least ? least : n;
-}
+// How a group is counted: in tiles of `rows` of its rows, the last one not full, at least `least` of them, and `extra`
+// (rows 0: each group is one unit).
+struct Units {
+  int rows, least, extra;
+  __device__ __forceinline__ long of(long n) const {
+    if (!rows) return 1;
+    const long u = (n + rows - 1) / rows;
+    return (u < least ? least : u) + extra;
+  }
+};
 
 // rows and units of all groups together
 struct Totals {
   long rows, units;
   bool valid;
 };
-__device__ __forceinline__ Totals count_groups(const float *sizes, int groups, int total, int unit, int least) {
+__device__ __forceinline__ Totals count_groups(const float *sizes, int groups, int total, Units unit) {
   Totals t{0, 0, true};
   for (int g0 = 0; g0 < groups && t.valid; g0 += kWave) {
     const int g = g0 + threadIdx.x % kWave;
     const float s = g < groups ? sizes[g] : 0.f;
     t.valid = !__any(!(s >= 0.f && s <= (float)total && s == floorf(s)));
-    long n = t.valid ? (long)s : 0, u = t.valid && g < groups ? units_of(n, unit, least) : 0;
+    long n = t.valid ? (long)s : 0, u = t.valid && g < groups ? unit.of(n) : 0;
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) {
       n += __shfl_xor(n, d, kWave);
@@ -172,12 +175,12 @@ struct Place {
   int first, count;
   long before;  // units of the groups in front
 };
-__device__ __forceinline__ Place locate(const float *sizes, int groups, int unit, int least, long want) {
+__device__ __forceinline__ Place locate(const float *sizes, int groups, Units unit, long want) {
   const int lane = threadIdx.x % kWave;
   long rows_before = 0, units_before = 0;
   for (int g0 = 0; g0 < groups; g0 += kWave) {
     const int g = g0 + lane;
-    const long n = g < groups ? (long)sizes[g] : 0, units = g < groups ? units_of(n, unit, least) : 0;
+    const long n = g < groups ? (long)sizes[g] : 0, units = g < groups ? unit.of(n) : 0;
     const long rows_in = wave_scan(n, lane), units_in = wave_scan(units, lane);
     const unsigned long long who = __ballot(want >= units_before + units_in - units && want < units_before + units_in);
     if (who) {
@@ -192,14 +195,14 @@ __device__ __forceinline__ Place locate(const float *sizes, int groups, int unit
 }
 
 // group `group`
-__device__ __forceinline__ Place locate_group(const float *sizes, int groups, int unit, int least, int group) {
+__device__ __forceinline__ Place locate_group(const float *sizes, int groups, Units unit, int group) {
   const int lane = threadIdx.x % kWave;
   long rows = 0, units = 0;
   for (int g0 = 0; g0 < group; g0 += kWave) {
     const int g = g0 + lane;
     const long n = g < group ? (long)sizes[g] : 0;
     rows += n;
-    units += g < group ? units_of(n, unit, least) : 0;
+    units += g < group ? unit.of(n) : 0;
   }
 #pragma unroll
   for (int d = kWave / 2; d > 0; d >>= 1) {
@@ -257,7 +260,7 @@ struct Work {
 };
 __device__ __forceinline__ Work whole_work(const Product &P, int tile_rows, int row_tile) { return Work{P.b, P.c, row_tile * tile_rows, P.m, 0, P.k}; }
 __device__ __forceinline__ Work rows_work(const Product &P, int tile_rows, long row_tile) {
-  const Place at = locate(P.sizes, P.groups, tile_rows, 0, row_tile);
+  const Place at = locate(P.sizes, P.groups, Units{tile_rows, 0, 0}, row_tile);
   const int group = uniform(at.group), skip = uniform((int)(row_tile - at.before)) * tile_rows, first = uniform(at.first), count = uniform(at.count);
   if (group < 0) return Work{P.b, P.c, 0, 0, 0, 0};
   return Work{P.b + group * P.b_g, P.c, first + skip, first + min(count, skip + tile_rows), 0, P.k};
@@ -267,8 +270,8 @@ __device__ __forceinline__ Work depth_work(const Product &P, int tile_rows, int 
   return Work{P.b, P.c + group * P.c_g, row_tile * tile_rows, P.m, first, first + count};
 }
 // false, and the host will hear of it: sizes that do not fit
-__device__ __forceinline__ bool check_groups(const Product &P, int unit, int least, bool first_block, long &units) {
-  const Totals t = count_groups(P.sizes, P.groups, P.ragged == ROWS ? P.m : P.k, unit, least);
+__device__ __forceinline__ bool check_groups(const Product &P, Units unit, bool first_block, long &units) {
+  const Totals t = count_groups(P.sizes, P.groups, P.ragged == ROWS ? P.m : P.k, unit);
   units = uniform(t.units);
   if (uniform((int)t.valid)) return true;
   if (threadIdx.x == 0 && first_block) *P.fault = kFaultGroups;
@@ -280,9 +283,9 @@ __device__ __forceinline__ bool find_work(const Product &P, int tile_rows, int r
     w = whole_work(P, tile_rows, row_tile);
   } else {
     long units;
-    if (!check_groups(P, P.ragged == ROWS ? tile_rows : 0, 0, first_block, units)) return false;
+    if (!check_groups(P, Units{P.ragged == ROWS ? tile_rows : 0, 0, 0}, first_block, units)) return false;
     if (P.ragged == ROWS) w = rows_work(P, tile_rows, row_tile);
-    else w = depth_work(P, tile_rows, row_tile, locate(P.sizes, P.groups, 0, 0, group));
+    else w = depth_work(P, tile_rows, row_tile, locate(P.sizes, P.groups, Units{0, 0, 0}, group));
   }
   return w.row0 < w.rows;
 }
@@ -423,9 +426,9 @@ struct Feed {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int START_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, TH = 64 * WM * WN;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, START = START_, TH = 64 * WM * WN;
   static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
 };
 
@@ -444,12 +447,14 @@ __device__ __forceinline__ void tile_of(long tile, int tiles_m, int tiles_n, int
 // in `work`, two places to a block, and add_parts adds them in the order of k and finishes the tile.  (Added by the
 // block that comes last, in the same launch, they cost more: one compute unit reads some 17 bytes per nanosecond, and
 // 1024^3 in 128 x 128 tiles took 59 us against 29.)
+// A tile counts as START slabs more than it has, its first loads and its epilogue: the blocks that got the tiles of small
+// groups would else be the last by far (weights' gradient of 4095 rows in 8 groups of 45 to 1200: 274 us).
 struct Sharing {
   int tiles_m, tiles_n, slabs;  // DEPTH: slabs is by group
   int rounds;
   long shared, run;             // tiles whose slabs are shared out, in runs of so many
 };
-template <int BM, int BN>
+template <int BM, int BN, int START>
 __device__ __forceinline__ bool share_out(const Product &P, int blocks, bool first_block, Sharing &h) {
   h.tiles_n = (P.n + BN - 1) / BN;
   h.tiles_m = (P.m + BM - 1) / BM;
@@ -457,16 +462,16 @@ __device__ __forceinline__ bool share_out(const Product &P, int blocks, bool fir
   h.rounds = 0;
   long units;
   if (P.ragged == DEPTH) {
-    if (!check_groups(P, KS, 1, first_block, units)) return false;
+    if (!check_groups(P, Units{KS, 1, START}, first_block, units)) return false;
     h.shared = (long)h.tiles_m * h.tiles_n * P.groups;
     units *= (long)h.tiles_m * h.tiles_n;
   } else {
-    if (!check_groups(P, BM, 0, first_block, units)) return false;
+    if (!check_groups(P, Units{BM, 0, 0}, first_block, units)) return false;
     h.tiles_m = (int)units;
     const long tiles = (long)h.tiles_m * h.tiles_n;
     h.rounds = (int)quotient(tiles, blocks);
     h.shared = tiles - (long)h.rounds * blocks;
-    units = h.shared * h.slabs;
+    units = h.shared * (h.slabs + START);
   }
   const long sharers = min((long)blocks, h.shared * P.most_sharers);
   h.run = sharers ? max(quotient(units + sharers - 1, sharers), 1l) : 1;
@@ -494,9 +499,9 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
   Sharing h;
   long u = 0, u_end = 0;
   if (RUNS) {
-    if (!share_out<T::BM, T::BN>(P, blocks, blockIdx.x == 0, h)) return;
+    if (!share_out<T::BM, T::BN, T::START>(P, blocks, blockIdx.x == 0, h)) return;
     u = uniform(me * h.run);
-    u_end = uniform(P.ragged == DEPTH ? u + h.run : min(u + h.run, h.shared * h.slabs));
+    u_end = uniform(P.ragged == DEPTH ? u + h.run : min(u + h.run, h.shared * (h.slabs + T::START)));
   } else {
     h = Sharing{(P.m + T::BM - 1) / T::BM, (P.n + T::BN - 1) / T::BN, (P.k + KS - 1) / KS, 1, 0, 1};
   }
@@ -510,21 +515,24 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
     if (RUNS && u < u_end) {
       if (P.ragged == DEPTH) {
         const long per_slab = (long)h.tiles_m * h.tiles_n;
-        const Place at = locate(P.sizes, P.groups, KS, 1, quotient(u, per_slab));
+        const Units unit{KS, 1, T::START};
+        const Place at = locate(P.sizes, P.groups, unit, quotient(u, per_slab));
         if (uniform(at.group) < 0) break;  // behind the last group
-        slabs = uniform((int)units_of(at.count, KS, 1));
+        slabs = uniform((int)unit.of(at.count)) - T::START;
         const long in = u - uniform(at.before) * per_slab;
-        tile = quotient(in, slabs);
-        s0 = (int)(in - tile * slabs);
+        tile = quotient(in, slabs + T::START);
+        unit0 = u - (in - tile * (slabs + T::START));
         tile_of(tile, h.tiles_m, h.tiles_n, tm, tn);
         w = depth_work(P, T::BM, tm, at);
       } else {
-        tile = quotient(u, slabs);
-        s0 = (int)(u - tile * slabs);
+        tile = quotient(u, slabs + T::START);
+        unit0 = tile * (slabs + T::START);
       }
-      unit0 = u - s0;
-      n = (int)min((long)(slabs - s0), u_end - u);
-      u += n;
+      const int p0 = (int)(u - unit0) - T::START, p1 = (int)(min(unit0 + T::START + slabs, u_end) - unit0) - T::START;
+      u += p1 - p0;
+      s0 = max(p0, 0);
+      n = max(p1, 0) - s0;
+      if (n == 0) continue;
     } else if (round < h.rounds) {
       tile = h.shared + (long)round * blocks + me;
       round++;
@@ -705,10 +713,10 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
 // The parts of the shared tiles, added in the order of k, and the epilogue: a block takes 16 rows of a tile
 // (blockIdx.y), a thread a column.
 constexpr int kAddRows = 16;
-template <int BM, int BN>
+template <int BM, int BN, int START>
 __global__ __launch_bounds__(256) void add_parts(Product P, int blocks) {
   Sharing h;
-  if (!share_out<BM, BN>(P, blocks, false, h)) return;
+  if (!share_out<BM, BN, START>(P, blocks, false, h)) return;
   const long index = blockIdx.x;
   if (index >= h.shared) return;
   int tm, tn, slabs = h.slabs;
@@ -716,17 +724,18 @@ __global__ __launch_bounds__(256) void add_parts(Product P, int blocks) {
   Work w;
   if (P.ragged == DEPTH) {
     const long tiles = (long)h.tiles_m * h.tiles_n, group = quotient(index, tiles), tile = index - group * tiles;
-    const Place at = locate_group(P.sizes, P.groups, KS, 1, (int)group);
-    slabs = uniform((int)units_of(at.count, KS, 1));
-    unit0 = uniform(at.before) * tiles + tile * slabs;
+    const Units unit{KS, 1, START};
+    const Place at = locate_group(P.sizes, P.groups, unit, (int)group);
+    slabs = uniform((int)unit.of(at.count)) - START;
+    unit0 = uniform(at.before) * tiles + tile * (slabs + START);
     tile_of(tile, h.tiles_m, h.tiles_n, tm, tn);
     w = depth_work(P, BM, tm, at);
   } else {
-    unit0 = index * slabs;
+    unit0 = index * (slabs + START);
     tile_of(index, h.tiles_m, h.tiles_n, tm, tn);
     w = rows_work(P, BM, tm);
   }
-  const long first = quotient(unit0, h.run), last = quotient(unit0 + slabs - 1, h.run);
+  const long first = quotient(unit0 + START, h.run), last = quotient(unit0 + START + slabs - 1, h.run);
   if (first == last) return;  // finished by the block that had all of it
   constexpr int ROWS_AT_ONCE = 256 / BN, N = kAddRows / ROWS_AT_ONCE;
   const int col = threadIdx.x % BN, row = blockIdx.y * kAddRows + threadIdx.x / BN;
@@ -966,7 +975,7 @@ constexpr int kSliceRows = 8;
 __global__ __launch_bounds__(256) void add_slices(Product P) {
   int rows = P.m;
   if (P.ragged == ROWS) {
-    const Totals t = count_groups(P.sizes, P.groups, P.m, 0, 0);
+    const Totals t = count_groups(P.sizes, P.groups, P.m, Units{0, 0, 0});
     if (!t.valid) return;
     rows = (int)t.rows;
   }
@@ -1044,6 +1053,7 @@ void check_launch(const char *what) {
 //                 chip, 234 TFLOP/s against 185 for 128 x 128 and 148 for 64 x 128 at 4096^3, and the worst on part
 //                 of one
 //   start         what a block's first loads and its epilogue cost, in slabs
+//   stream        the operands' bytes, of which the tiles get 3.5 TB/s
 //   adding        the launch that adds the parts of shared tiles costs 4.8 us and its bytes
 // Up to 64 rows the kernel for few rows takes part, with what a block of 16 to 64 rows reads per nanosecond (`alone`)
 // and what the chip reaches (1 x 4096 x 16384: 46 us, in tiles 64).
@@ -1078,7 +1088,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
     if (ft && atoi(ft) != t + 1) continue;
     const TileCost &c = kTiles[t];
     const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
-    const double slabs = std::fmax(std::ceil(k / KS), 1.);
+    const double slabs = std::fmax(std::ceil(k / KS), 1.), stream = 4. * ((double)P.m * P.k + (double)P.k * P.n + outputs) / 3500e3 * share;
     auto busy = [&](double per) {  // a block's time per slab with `per` blocks to a compute unit
       if (per <= 1) return c.resident > 1 ? c.alone : c.alone + (c.full - c.alone) * per;
       return c.alone + (c.full - c.alone) * (per - 1) / (c.resident - 1);
@@ -1091,14 +1101,15 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
         const double per = tiles * s * share / 256., whole = per > 1 ? std::ceil(per) : per;
         const double turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
         double us = 4.1 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (std::ceil(slabs / s) + c.start);
+        us = std::fmax(us, 4.1 + stream);
         if (s > 1) us += 4.8 + 4. * outputs * (2 * s + 1) / 13800e3;
         consider(ThclProductPlan{t, 1, 1, s}, us);
       } else {
         const int blocks = (int)std::fmin((double)cus * c.resident, std::ceil(tiles) * s);
         const double rounds = P.ragged == DEPTH ? 0. : std::floor(tiles / blocks), shared = tiles - rounds * blocks;
-        const double sharers = std::fmin(blocks, shared * s), run = std::ceil(shared * slabs / sharers);
+        const double sharers = std::fmin(blocks, shared * s), run = std::ceil(shared * (slabs + c.start) / sharers);
         double us = 5.5 + rounds * busy(std::ceil(blocks * share / 256.)) * (slabs + c.start);
-        if (shared > 0) us += busy(std::ceil(sharers * share / 256.)) * (run + c.start);
+        if (shared > 0) us += busy(std::ceil(sharers * share / 256.)) * run;
         // the parts are written and read, the tiles written
         if (P.ragged == DEPTH || s > 1) us += 4.8 + 4. * c.bm * c.bn * (2 * sharers + shared) / 13800e3;
         consider(ThclProductPlan{t, blocks, s, 1}, us);
@@ -1143,7 +1154,7 @@ static void launch_split(const Product &P, bool akc, bool bkc, int blocks, hipSt
   // the tiles that may have been shared
   const long shared = P.ragged == DEPTH ? tiles_m * tiles_n * P.groups : blocks;
   THCL_CHECK(shared <= INT32_MAX, THCL_DIM_WARNING);
-  hipLaunchKernelGGL((add_parts<T::BM, T::BN>), dim3((unsigned)shared, T::BM / kAddRows), dim3(256), 0, stream, P, blocks);
+  hipLaunchKernelGGL((add_parts<T::BM, T::BN, T::START>), dim3((unsigned)shared, T::BM / kAddRows), dim3(256), 0, stream, P, blocks);
   check_launch(what);
 }
 template <int MT>
@@ -1184,10 +1195,10 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
     THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
   }
   switch (plan.kind) {
-    case 0: launch_split<Tile<256, 256, 2, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 1: launch_split<Tile<128, 128, 2, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 2: launch_split<Tile<64, 128, 2, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 3: launch_split<Tile<32, 128, 1, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 0: launch_split<Tile<256, 256, 2, 4, 7>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 1: launch_split<Tile<128, 128, 2, 2, 6>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 2: launch_split<Tile<64, 128, 2, 2, 3>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 3: launch_split<Tile<32, 128, 1, 4, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
     case 4: launch_thin<1>(P, bkc, row_tiles(16), stream, what); break;
     case 5: launch_thin<2>(P, bkc, row_tiles(32), stream, what); break;
     case 6: launch_thin<3>(P, bkc, row_tiles(48), stream, what); break;
