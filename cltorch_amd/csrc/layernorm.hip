@@ -276,8 +276,7 @@ __global__ __launch_bounds__(kFoldRuns *kFoldCols) void norm_fold(NormGradParams
 
 // ------------------------------------------------ rows that do not fit registers ---
 constexpr int kWide = 1024;
-__global__ __launch_bounds__(kWide) void norm_wide(NormParams P) {
-  const long row = blockIdx.x;
+__device__ __forceinline__ void norm_wide_row(const NormParams &P, long row) {
   const float *x = P.x + row * P.x_pitch;
   float *y = P.y + row * P.y_pitch;
   double s = 0.0, none = 0.0;
@@ -302,9 +301,11 @@ __global__ __launch_bounds__(kWide) void norm_wide(NormParams P) {
     if (P.rstd) P.rstd[row] = rstd;
   }
 }
+__global__ __launch_bounds__(kWide) void norm_wide(NormParams P) {
+  for (long row = blockIdx.x; row < P.rows; row += gridDim.x) norm_wide_row(P, row);
+}
 
-__global__ __launch_bounds__(kWide) void norm_grad_wide(NormGradParams P) {
-  const long row = blockIdx.x;
+__device__ __forceinline__ void norm_grad_wide_row(const NormGradParams &P, long row) {
   const float *x = P.x + row * P.x_pitch, *gy = P.gy + row * P.gy_pitch;
   float *gx = P.gx + row * P.gx_pitch;
   const float mean = P.mean[row], rstd = P.rstd[row];
@@ -325,7 +326,19 @@ __global__ __launch_bounds__(kWide) void norm_grad_wide(NormGradParams P) {
   }
 }
 
-__global__ __launch_bounds__(kWide) void norm_grad_columns(NormGradParams P) { norm_columns<kWide>(P, blockIdx.x); }
+__global__ __launch_bounds__(kWide) void norm_grad_wide(NormGradParams P) {
+  for (long row = blockIdx.x; row < P.rows; row += gridDim.x) norm_grad_wide_row(P, row);
+}
+
+__global__ __launch_bounds__(kWide) void norm_grad_columns(NormGradParams P) {
+  for (long block = blockIdx.x; 32 * block < P.width; block += gridDim.x) {
+    norm_columns<kWide>(P, block);
+    __syncthreads();  // its sums have been read
+  }
+}
+
+// a launch's threads are counted in 32 bits: at most so many blocks, which walk over what there is
+unsigned blocks_of(long n) { return (unsigned)(n < 1l << 20 ? n : 1l << 20); }
 
 void check_launch(const char *what) {
   const hipError_t e = hipGetLastError();
@@ -381,7 +394,7 @@ void thcl_norm(THClState *state, thcl_rt *rt, const NormParams &P) {
     fits = few && by_width(P.width, go, Choice<16, 4, 64, 4, 256, 4, 256, 8, 256, 16>{});
     fits = fits || by_width(P.width, go, Choice<16, 4, 16, 8, 64, 4, 64, 8, 64, 16, 256, 8, 256, 16, 1024, 8>{});
   }
-  if (!fits) hipLaunchKernelGGL(norm_wide, dim3((unsigned)P.rows), dim3(kWide), 0, stream, P);
+  if (!fits) hipLaunchKernelGGL(norm_wide, dim3(blocks_of(P.rows)), dim3(kWide), 0, stream, P);
   check_launch("layerNorm");
   thcl_after_launch(state, rt);
 }
@@ -431,9 +444,9 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
     if (P.parts) hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * P.width + kFoldCols - 1) / kFoldCols)), dim3(kFoldRuns * kFoldCols), 0, stream, P, (int)blocks);
   } else {
     if (columns)  // first: gx may take the place of gy or x
-      hipLaunchKernelGGL(norm_grad_columns, dim3((unsigned)((P.width + 31) / 32)), dim3(kWide), 0, stream, P);
+      hipLaunchKernelGGL(norm_grad_columns, dim3(blocks_of((P.width + 31) / 32)), dim3(kWide), 0, stream, P);
     check_launch("layerNormBackward");
-    if (P.gx) hipLaunchKernelGGL(norm_grad_wide, dim3((unsigned)P.rows), dim3(kWide), 0, stream, P);
+    if (P.gx) hipLaunchKernelGGL(norm_grad_wide, dim3(blocks_of(P.rows)), dim3(kWide), 0, stream, P);
   }
   check_launch("layerNormBackward");
   thcl_after_launch(state, rt);

@@ -54,7 +54,8 @@ Shape shape2(long a, long b) {
   s.size[1] = b;
   return s;
 }
-void check_int(long v) { THCL_CHECK(v <= INT32_MAX, THCL_DIM_WARNING); }
+// the kernels count rows and columns in 32 bits, a tile beyond the last one included
+void check_int(long v) { THCL_CHECK(v <= INT32_MAX - 65536, THCL_DIM_WARNING); }
 }  // namespace
 
 extern "C" {

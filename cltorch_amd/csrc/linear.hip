@@ -7,7 +7,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -413,15 +412,15 @@ struct Feed {
         *(u4 *)(lds + to[o] + p * S::PART) = part;
       }
   }
-  // the last slab: kleft values of k are the operand's; those behind belong to the next line
+  // the last slab: kleft values of k are the operand's; those behind belong to the next line, or, where lines share
+  // memory (a pitch of zero), lie in front of the buffer's end
   __device__ __forceinline__ void store_last(char *lds, float (&x)[N][8], int kleft) {
 #pragma unroll
-    for (int o = 0; o < N; o++)
-      if (KC) {
-        const int chunk = (threadIdx.x + TH * o) % CHUNKS;
+    for (int o = 0; o < N; o++) {
+      const int f = (threadIdx.x + TH * o) % OCTETS, chunk = KC ? f % CHUNKS : f / LINES;
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[o][e] = 8 * chunk + e < kleft ? x[o][e] : 0.f;
-      }
+      for (int e = 0; e < 8; e++) x[o][e] = 8 * chunk + e < kleft ? x[o][e] : 0.f;
+    }
     store(lds, x);
   }
 };
@@ -441,12 +440,13 @@ __device__ __forceinline__ void tile_of(long tile, int tiles_m, int tiles_n, int
   tn = uniform((int)((unsigned)in / (unsigned)down));
   tm = uniform(8 * g + in - tn * down);
 }
-// Ragged products: as many blocks as the compute units hold share the slabs of all tiles evenly.  Whole rounds of tiles go to the blocks
-// as they are, and the slabs of the tiles that remain (all of them, when they are fewer than blocks) are cut into equal
-// runs, each a part of one tile or the end of one and the beginning of the next.  The blocks of a tile leave their sums
-// in `work`, two places to a block, and add_parts adds them in the order of k and finishes the tile.  (Added by the
-// block that comes last, in the same launch, they cost more: one compute unit reads some 17 bytes per nanosecond, and
-// 1024^3 in 128 x 128 tiles took 59 us against 29.)
+
+// Ragged products: as many blocks as the compute units hold share the slabs of all tiles evenly.  Whole rounds of tiles
+// go to the blocks as they are, and the slabs of the tiles that remain (all of them, when they are fewer than blocks,
+// and DEPTH) are cut into equal runs, each a part of one tile or the end of one and the beginning of the next.  The
+// blocks of a tile leave their sums in `work`, two places to a block, and add_parts adds them in the order of k and
+// finishes the tile.  (Added by the block that comes last, in the same launch, they cost more: one compute unit reads
+// some 17 bytes per nanosecond, and 1024^3 in 128 x 128 tiles took 59 us against 29.)
 // A tile counts as START slabs more than it has, its first loads and its epilogue: the blocks that got the tiles of small
 // groups would else be the last by far (weights' gradient of 4095 rows in 8 groups of 45 to 1200: 274 us).
 struct Sharing {
@@ -805,14 +805,15 @@ struct ThinStream {
 #pragma unroll
         for (int t = 0; t < MT; t++) x[t][e] = 8 * g + e < kleft ? x[t][e] : 0.f;
     }
+    if (LAST) {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[i][e] = (BKC ? 4 * (lane % 8) + e : 8 * g + i) < kleft ? y[i][e] : 0.f;
+    }
     if (BKC) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (LAST)
-#pragma unroll
-          for (int e = 0; e < 4; e++) y[i][e] = 4 * (lane % 8) + e < kleft ? y[i][e] : 0.f;
-        *(f4 *)(turn + (8 * i + lane / 8) * PITCH + 4 * (lane % 8)) = y[i];
-      }
+      for (int i = 0; i < 8; i++) *(f4 *)(turn + (8 * i + lane / 8) * PITCH + 4 * (lane % 8)) = y[i];
     }
     u4 pa[MT][3];
     if constexpr (SPLIT) {
@@ -1023,22 +1024,28 @@ __global__ __launch_bounds__(256) void slope_columns(SlopeParams P) {
 __global__ __launch_bounds__(256) void slope_fold(SlopeParams P, int parts) {
   __shared__ double sums[16][16];
   const int lane = threadIdx.x % 16, run = threadIdx.x / 16;
-  const long col = (long)blockIdx.x * 16 + lane;
   const int p0 = (int)((long)parts * run / 16), p1 = (int)((long)parts * (run + 1) / 16);
-  double s = 0.0;
-  if (col < P.width)
+  for (long col0 = (long)blockIdx.x * 16; col0 < P.width; col0 += (long)gridDim.x * 16) {
+    const long col = col0 + lane;
+    double s = 0.0;
+    if (col < P.width)
 #pragma unroll 8
-    for (int p = p0; p < p1; p++) s += P.parts[p * P.width + col];
-  sums[run][lane] = s;
-  __syncthreads();
-  if (run != 0 || col >= P.width) return;
+      for (int p = p0; p < p1; p++) s += P.parts[p * P.width + col];
+    sums[run][lane] = s;
+    __syncthreads();
+    if (run == 0 && col < P.width) {
 #pragma unroll
-  for (int i = 1; i < 16; i++) s += sums[i][lane];
-  P.gb[col * P.gb_step] = (float)s;
+      for (int i = 1; i < 16; i++) s += sums[i][lane];
+      P.gb[col * P.gb_step] = (float)s;
+    }
+    __syncthreads();  // the sums have been read
+  }
 }
 
 // an operand's pitch from which a tile's lines no longer fit 32-bit byte offsets
 constexpr long kFarPitch = 1l << 21;
+// a launch's threads along a dimension of the grid are counted in 32 bits: blocks of up to 1024, far below that
+constexpr long kMostBlocks = 1l << 20;
 
 void check_launch(const char *what) {
   const hipError_t e = hipGetLastError();
@@ -1083,9 +1090,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
     if (P.ragged != ROWS) return (double)((P.m + rows - 1) / rows);
     return P.m <= (double)rows * groups ? (double)groups : (double)P.m / rows + 0.5 * groups;
   };
-  const char *ft = getenv("THCL_TILE"), *fs = getenv("THCL_SLICES");
   for (int t = 0; t < 4; t++) {
-    if (ft && atoi(ft) != t + 1) continue;
     const TileCost &c = kTiles[t];
     const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
     const double slabs = std::fmax(std::ceil(k / KS), 1.), stream = 4. * ((double)P.m * P.k + (double)P.k * P.n + outputs) / 3500e3 * share;
@@ -1094,7 +1099,6 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
       return c.alone + (c.full - c.alone) * (per - 1) / (c.resident - 1);
     };
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {  // blocks to a tile
-      if (fs && atoi(fs) != s) continue;
       if (s > 1 && slabs / s < 4) break;
       if (P.ragged == WHOLE) {
         if (s > 1 && s * outputs * 4 > 1e9) break;
@@ -1116,7 +1120,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
       }
     }
   }
-  if (few_rows_fit && !ft) {
+  if (few_rows_fit) {
     const double rows = P.ragged == ROWS ? (double)P.m / groups : P.m;
     // a group may hold more than the average: half as much again still fits the tile
     const int mt = (int)std::ceil(rows * (P.ragged == ROWS ? 1.5 : 1.) / 16);
@@ -1183,7 +1187,7 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
     thcl_after_launch(state, rt);
     return;
   }
-  const bool thin = akc && P.ragged != DEPTH && row_tiles(16) <= 65535;
+  const bool thin = akc && P.ragged != DEPTH && row_tiles(16) <= 65535 && P.n / kThinCols < kMostBlocks;
   const ThclProductPlan plan = thcl_product_plan(P, thin, thcl_rt_get_props(rt)->compute_units);
   P.most_sharers = plan.most_sharers;
   P.slices = plan.slices;
@@ -1236,7 +1240,8 @@ void thcl_slope(THClState *state, thcl_rt *rt, const SlopeParams &given) {
 #undef GO
   check_launch("linearBackward");
   if (P.gb) {
-    hipLaunchKernelGGL(slope_fold, dim3((unsigned)((P.width - 1) / 16 + 1)), dim3(256), 0, stream, P, (int)parts);
+    const long fold = (P.width - 1) / 16 + 1;
+    hipLaunchKernelGGL(slope_fold, dim3((unsigned)(fold < kMostBlocks ? fold : kMostBlocks)), dim3(256), 0, stream, P, (int)parts);
     check_launch("linearBackward");
   }
   thcl_after_launch(state, rt);

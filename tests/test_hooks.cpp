@@ -7,6 +7,7 @@
 #include <string>
 
 #include "internal.h"
+#include "layers.h"
 
 extern "C" {
 static void dbg_header(THClTensor &h, int nd, long *sz, long *st, long off) {
@@ -107,6 +108,14 @@ unsigned thcl_dbg_divide(unsigned n, long d) { return thcl_host_divide(n, d); }
 
 void thcl_dbg_gemm_plan(long m, long n, long k, int cus, int *bm, int *bn, int *ksplit, int *kchunk, int *tail_tiles, int *tail_split) {
   thcl_gemm_plan(m, n, k, cus, bm, bn, ksplit, kchunk, tail_tiles, tail_split);
+}
+
+// plan: kind, blocks, most_sharers, slices
+void thcl_dbg_product_plan(int ragged, int m, int n, int k, int groups, int few_rows_fit, int cus, int *plan) {
+  Product P = {};
+  P.ragged = ragged, P.m = m, P.n = n, P.k = k, P.groups = groups;
+  const ThclProductPlan got = thcl_product_plan(P, few_rows_fit != 0, cus);
+  plan[0] = got.kind, plan[1] = got.blocks, plan[2] = got.most_sharers, plan[3] = got.slices;
 }
 #endif
 }

@@ -32,6 +32,21 @@ def test_tensor_bookkeeping_under_sanitizers(tmp_path):
 
 
 @pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not found")
+def test_layer_entry_points_under_sanitizers(tmp_path):
+    """cltorch_amd/csrc/layers.cpp with plain loops in place of its kernels: views, stand-ins, in-place forms and
+    refusals of layer norm, linear layer and grouped products."""
+    exe = str(tmp_path / "host_layers_check")
+    cmd = SAN + [os.path.join(ROOT, "tests", "host_layers_check.cpp"), os.path.join(ROOT, "tests", "host_rt_stub.cpp"),
+                 os.path.join(CSRC, "layers.cpp"), os.path.join(CSRC, "tensor.cpp"), os.path.join(CSRC, "state.cpp"),
+                 os.path.join(CSRC, "layout.cpp"), "-o", exe]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([exe, "400"], capture_output=True, text=True, env=ENV, timeout=300)
+    assert r.returncode == 0, (r.stdout + r.stderr)[-3000:]
+    assert "rounds of layers ok" in r.stdout
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not found")
 def test_layout_and_rewrite_under_sanitizers(tmp_path):
     inc = os.path.join(CSRC, "apply_device_src.inc")
     if not os.path.exists(inc):                      # generated by the library build
