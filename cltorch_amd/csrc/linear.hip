@@ -345,21 +345,27 @@ struct Staged {
   }
 };
 
-// An operand on its way to LDS.  KC: contiguous along k (lanes take octets of k of a line, two lanes a line);
-// otherwise contiguous along its lines (lanes take neighbouring lines, eight k each).  Loads go through a buffer
-// descriptor that begins at the slab and ends behind the last element, so what lies behind reads as zero.
+// An operand on its way to LDS, E values of k of a line at a time, 8 or, where that leaves threads without any, 4.  KC:
+// contiguous along k (lanes take neighbouring pieces of a line); otherwise contiguous along its lines (lanes take
+// neighbouring lines).  Loads go through a buffer descriptor that begins at the slab and ends behind the last element, so
+// what lies behind reads as zero.
 template <int LINES, int IL, bool KC, int TH>
 struct Feed {
   typedef Staged<LINES, IL> S;
-  static constexpr int OCTETS = LINES * CHUNKS;
-  static constexpr int N = OCTETS >= TH ? OCTETS / TH : 1;
+  static constexpr int E = LINES * KS / 8 >= TH ? 8 : 4, PER_LINE = KS / E, PIECES = LINES * PER_LINE;
+  static constexpr int N = PIECES >= TH ? PIECES / TH : 1;
+  typedef unsigned Part __attribute__((ext_vector_type(E / 2)));
   const char *base;       // the slab that is loaded next
   long left;              // bytes from there to behind the last element; what is not positive reads as zero
   long step;
   unsigned off[N];
   int row_bytes;          // along k, when the lines are contiguous
-  int to[N];              // where the octet goes in LDS
+  int to[N];              // where the piece goes in LDS
   unsigned least = ~0u;   // smallest magnitude met: its bits shifted up by one, less one (zero counts as the largest)
+  static __device__ __forceinline__ int piece(int i) {
+    const int f = (threadIdx.x + TH * i) % PIECES;  // threads beyond the last piece repeat one: no branch around loads
+    return KC ? f % PER_LINE : f / LINES;
+  }
   __device__ __forceinline__ void begin(const float *p, long line_stride, long k_stride, int line0, int lines, int k0, int k1) {
     const long have = min(lines - line0, LINES);
     base = (const char *)uniform((long)(p + (long)line0 * line_stride + (long)k0 * k_stride));
@@ -368,13 +374,12 @@ struct Feed {
     row_bytes = (int)(4 * k_stride);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int f = (threadIdx.x + TH * i) % OCTETS;  // threads beyond the last octet repeat one: no branch around loads
-      const int line = KC ? f / CHUNKS : f % LINES, chunk = KC ? f % CHUNKS : f / LINES;
-      off[i] = (unsigned)(4 * (line * line_stride + 8l * chunk * k_stride));
-      to[i] = S::at(line, chunk);
+      const int f = (threadIdx.x + TH * i) % PIECES, line = KC ? f / PER_LINE : f % LINES, k = E * piece(i);
+      off[i] = (unsigned)(4 * (line * line_stride + k * k_stride));
+      to[i] = S::at(line, k / 8) + k % 8 * 2;
     }
   }
-  __device__ __forceinline__ void load(float (&x)[N][8]) {
+  __device__ __forceinline__ void load(float (&x)[N][E]) {
     const long l = left < 0 ? 0 : left > 0xffffffffl ? 0xffffffffl : left;
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)l, 0x00020000);
     base += step;
@@ -382,24 +387,26 @@ struct Feed {
 #pragma unroll
     for (int i = 0; i < N; i++) {
       if (KC) {
-        const f4 a = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i], 0, 0));
-        const f4 b = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i] + 16, 0, 0));
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
+        for (int q = 0; q < E / 4; q++) {
+          const f4 a = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i] + 16 * q, 0, 0));
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[i][4 * q + e] = a[e];
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off[i], e * row_bytes, 0));
+        for (int e = 0; e < E; e++) x[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off[i], e * row_bytes, 0));
       }
     }
   }
-  __device__ __forceinline__ void store(char *lds, float (&x)[N][8]) {
+  __device__ __forceinline__ void store(char *lds, float (&x)[N][E]) {
 #pragma unroll
     for (int o = 0; o < N; o++)
 #pragma unroll
       for (int p = 0; p < 3; p++) {
-        u4 part;
+        Part part;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < E / 2; i++) {
           float &a = x[o][2 * i], &b = x[o][2 * i + 1];
           if (p == 0) least = min(least, min((__float_as_uint(a) << 1) - 1u, (__float_as_uint(b) << 1) - 1u));
           const unsigned v = round_pair(a, b);
@@ -409,25 +416,28 @@ struct Feed {
             b -= __uint_as_float(v & 0xffff0000u);
           }
         }
-        *(u4 *)(lds + to[o] + p * S::PART) = part;
+        *(Part *)(lds + to[o] + p * S::PART) = part;
       }
   }
   // the last slab: kleft values of k are the operand's; those behind belong to the next line, or, where lines share
   // memory (a pitch of zero), lie in front of the buffer's end
-  __device__ __forceinline__ void store_last(char *lds, float (&x)[N][8], int kleft) {
+  __device__ __forceinline__ void store_last(char *lds, float (&x)[N][E], int kleft) {
 #pragma unroll
-    for (int o = 0; o < N; o++) {
-      const int f = (threadIdx.x + TH * o) % OCTETS, chunk = KC ? f % CHUNKS : f / LINES;
+    for (int o = 0; o < N; o++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[o][e] = 8 * chunk + e < kleft ? x[o][e] : 0.f;
-    }
+      for (int e = 0; e < E; e++) x[o][e] = E * piece(o) + e < kleft ? x[o][e] : 0.f;
     store(lds, x);
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int START_>
+// BM x BN results by WM x WN waves, START: slabs that its first loads and its epilogue are worth.  Two waves or more to
+// a SIMD, so that one's matrix instructions run under the vector instructions with which another splits its operands:
+// 128 x 128 by eight waves with 4 values of k each takes 50 us for 1531 x 1027 x 2053, by four with 8 it took 61; 64 x
+// 128 by eight waves loses, 59 us against 55 at 1536 x 1024 x 2048.
+template <int BM_, int BN_, int WM_, int WN_, int START_, int SIMD_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, START = START_, TH = 64 * WM * WN;
+  static constexpr int SIMD = SIMD_;  // waves that have to fit a SIMD's registers
   static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
 };
 
@@ -486,7 +496,7 @@ __device__ __forceinline__ float *part_of(const Product &P, const Sharing &h, lo
 // RUNS: the ragged products, whose tiles the host cannot count; others have a block to each tile and slice of k, which
 // starts sooner (1000 x 64 x 64: 6.6 us against 8.0) and leaves whole rows of partial results.
 template <class T, bool AKC, bool BKC, bool RUNS>
-__global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
+__global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
   constexpr int MT = T::MT, NT = T::NT;
   typedef Feed<T::BM, MT, AKC, T::TH> FA;
   typedef Feed<T::BN, NT, BKC, T::TH> FB;
@@ -559,7 +569,7 @@ __global__ __launch_bounds__(T::TH, 2) void product_split(Product P) {
     fb.begin(w.b, P.b_n, P.b_k, col0, P.n, w.k0, w.k1);
     const int row0 = w.row0 + (wave / T::WN) * 32 * MT, wcol0 = col0 + (wave % T::WN) * 32 * NT;
     const int depth = w.k1 - w.k0, steps = (depth + KS - 1) / KS;
-    float xa[2][FA::N][8], xb[2][FB::N][8];
+    float xa[2][FA::N][FA::E], xb[2][FB::N][FB::E];
     f16v acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -1056,9 +1066,9 @@ void check_launch(const char *what) {
 // The kernel for a product, by a small model of the launch in microseconds on 256 compute units, fitted to 25 shapes of
 // 1000 x 64 x 64 to 4096^3:
 //   alone, full   a block's time per slab of 16 k when it has its compute unit to itself, and when `resident` of them
-//                 share one (128 x 128: 0.81 us for one block, 1.33 for two).  The largest tile is the best on a whole
-//                 chip, 234 TFLOP/s against 185 for 128 x 128 and 148 for 64 x 128 at 4096^3, and the worst on part
-//                 of one
+//                 share one (128 x 128: 0.62 us for one block, 1.28 for two).  The largest tile is the best on a whole
+//                 chip, 227 TFLOP/s against 190 for 128 x 128 and 162 for 64 x 128 at 4096^3, and the worst on part
+//                 of one, 68 us against 50 and 60 for 1531 x 1027 x 2053
 //   start         what a block's first loads and its epilogue cost, in slabs
 //   stream        the operands' bytes, of which the tiles get 3.5 TB/s
 //   adding        the launch that adds the parts of shared tiles costs 4.8 us and its bytes
@@ -1069,7 +1079,7 @@ struct TileCost {
   int bm, bn, resident;
   double alone, full, start;
 };
-constexpr TileCost kTiles[4] = {{256, 256, 1, 1.48, 2.09, 6.9}, {128, 128, 2, 0.81, 1.33, 5.5}, {64, 128, 3, 0.60, 1.28, 3.3}, {32, 128, 4, 0.53, 1.34, 1.7}};
+constexpr TileCost kTiles[4] = {{256, 256, 1, 1.51, 2.07, 7.8}, {128, 128, 2, 0.62, 1.28, 4.0}, {64, 128, 3, 0.51, 1.14, 4.1}, {32, 128, 4, 0.43, 1.11, 2.2}};
 struct ThinCost {
   double alone, chip;  // bytes per nanosecond
 };
@@ -1104,9 +1114,9 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
         if (s > 1 && s * outputs * 4 > 1e9) break;
         const double per = tiles * s * share / 256., whole = per > 1 ? std::ceil(per) : per;
         const double turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
-        double us = 4.1 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (std::ceil(slabs / s) + c.start);
-        us = std::fmax(us, 4.1 + stream);
-        if (s > 1) us += 4.8 + 4. * outputs * (2 * s + 1) / 13800e3;
+        double us = 4.4 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (std::ceil(slabs / s) + c.start);
+        us = std::fmax(us, 4.4 + stream);
+        if (s > 1) us += 4.8 + 4. * outputs * (2 * s + 1) / 14700e3;
         consider(ThclProductPlan{t, 1, 1, s}, us);
       } else {
         const int blocks = (int)std::fmin((double)cus * c.resident, std::ceil(tiles) * s);
@@ -1130,7 +1140,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
       for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (s > 1 && (k < 2 * kThinStep * kThinWaves * s || s * outputs * 4 > 1e9)) break;
         const double rate = std::fmin(tiles * s * c.alone, c.chip / share);
-        consider(ThclProductPlan{4 + mt - 1, 1, 1, s}, 4.5 + bytes / rate / 1e3 + (s > 1 ? 4.8 + 4. * outputs * (2 * s + 1) / 13800e3 : 0.));
+        consider(ThclProductPlan{4 + mt - 1, 1, 1, s}, 4.5 + bytes / rate / 1e3 + (s > 1 ? 4.8 + 4. * outputs * (2 * s + 1) / 14700e3 : 0.));
       }
     }
   }
@@ -1199,10 +1209,10 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
     THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
   }
   switch (plan.kind) {
-    case 0: launch_split<Tile<256, 256, 2, 4, 7>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 1: launch_split<Tile<128, 128, 2, 2, 6>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 2: launch_split<Tile<64, 128, 2, 2, 3>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 3: launch_split<Tile<32, 128, 1, 4, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 0: launch_split<Tile<256, 256, 2, 4, 7, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 1: launch_split<Tile<128, 128, 2, 4, 4, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 2: launch_split<Tile<64, 128, 2, 2, 4, 3>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 3: launch_split<Tile<32, 128, 1, 4, 2, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
     case 4: launch_thin<1>(P, bkc, row_tiles(16), stream, what); break;
     case 5: launch_thin<2>(P, bkc, row_tiles(32), stream, what); break;
     case 6: launch_thin<3>(P, bkc, row_tiles(48), stream, what); break;
