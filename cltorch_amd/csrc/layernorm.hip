@@ -45,10 +45,10 @@ __device__ __forceinline__ void row_sums(double &a, double &b) {
 // The elements a thread holds of a row: J units of V neighbouring ones, SPAN units apart.  V 4: a width that is a
 // multiple of 4, and results at addresses that are multiples of 16 bytes (loads need no alignment).  STREAM: past the
 // caches, for tensors that do not fit them (16384 x 4096 forward: 105 -> 99 us; 2047 x 1537 would lose, 9.8 -> 10.3).
-template <int SPAN, int V, int J, bool STREAM>
+template <int SPAN, int V, int J, bool STREAM, int LEAST = 256>
 struct Held {
   static constexpr int N = J * V;
-  static constexpr int LANES = SPAN < 256 ? 256 : SPAN;  // a block's threads; narrow rows go several to a block
+  static constexpr int LANES = SPAN < LEAST ? LEAST : SPAN;  // a block's threads; narrow rows go several to a block
   static constexpr int ROWS = LANES / SPAN;
   static __device__ __forceinline__ int first() { return ((int)threadIdx.x % SPAN) * V; }
   static __device__ __forceinline__ int at(int j) { return first() + j * SPAN * V; }
@@ -167,10 +167,16 @@ __device__ __forceinline__ void norm_columns(const NormGradParams &P, long block
   if (P.gb) P.gb[col * P.gb_step] = (float)sb;
 }
 
+// Rows that fit the caches are walked over by blocks of 512 threads at least, one to a compute unit, which leave half as
+// many parts of gw and gb as blocks of 256, two to a compute unit (2000 x 4096: 29.0 us against 33.2, 2047 x 1537: 17.8
+// against 18.8); rows past the caches by the latter, which are not held up by one another's sums (16384 x 4096: 143 us
+// against 160).
+template <int SPAN, int V, int J, bool STREAM, bool FEW>
+using HeldGrad = Held<SPAN, V, J, STREAM, FEW || STREAM ? 256 : 512>;
 // FEW rows: the first row_blocks blocks walk over the rows, the others sum columns, from the caches; nothing is folded.
 template <int SPAN, int V, int J, bool STREAM, bool FEW>
-__global__ __launch_bounds__(SPAN < 256 ? 256 : SPAN) void norm_grad(NormGradParams P, int row_blocks) {
-  typedef Held<SPAN, V, J, STREAM> H;
+__global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, FEW>::LANES)) void norm_grad(NormGradParams P, int row_blocks) {
+  typedef HeldGrad<SPAN, V, J, STREAM, FEW> H;
   if constexpr (FEW) {
     if ((int)blockIdx.x >= row_blocks) {
       norm_columns<H::LANES>(P, blockIdx.x - row_blocks);
@@ -406,15 +412,15 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
   const bool past = 12 * P.rows * P.width > kStreamBytes, columns = P.gw || P.gb;
   // Up to 1024 rows a second look at them from the caches is cheaper than the blocks' parts of gw and gb, which are then
   // as large as the rows, and a second launch (500 x 4096: 10.6 us against 26.7, 1000 x 4096: 19.4 against 27.5,
-  // 2000 x 4096: 41 against 34).
-  const bool few = P.rows <= 1024;
+  // 2000 x 4096: 41 against 29).  Without gw and gb there is nothing to leave.
+  const bool few = P.rows <= 1024 || (!columns && !past);
   long blocks = 0;
   auto with = [&](auto v) {
     return [&](auto span, auto j) {
       constexpr int SPAN = decltype(span)::value, V = decltype(v)::value, J = decltype(j)::value;
-      typedef Held<SPAN, V, J, false> H;
-      const long want = (P.rows + H::ROWS - 1) / H::ROWS;
       if (few) {
+        typedef HeldGrad<SPAN, V, J, false, true> H;
+        const long want = (P.rows + H::ROWS - 1) / H::ROWS;
         const long rows = P.gx ? want : 0, cols = columns ? (P.width + (H::LANES == 256 ? 16 : 32) - 1) / (H::LANES == 256 ? 16 : 32) : 0;
         auto launch = [&](long r, long c) {
           if (r + c > 0) hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, true>), dim3((unsigned)(r + c)), dim3(H::LANES), 0, stream, P, (int)r);
@@ -423,13 +429,14 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
         else launch(rows, cols);
         return;
       }
-      const long most = (long)cus * (H::LANES > 256 ? 1 : 2);
+      const int lanes = past ? HeldGrad<SPAN, V, J, true, false>::LANES : HeldGrad<SPAN, V, J, false, false>::LANES;
+      const long want = (P.rows + lanes / SPAN - 1) / (lanes / SPAN), most = (long)cus * (lanes > 256 ? 1 : 2);
       blocks = want < most ? want : most;
       if (columns) {
         P.parts = (double *)thcl_rt_workspace(rt, (size_t)blocks * 2 * P.width * sizeof(double));
         THCL_CHECK(P.parts != nullptr, "layerNormBackward workspace: %s", thcl_rt_error());
       }
-      const dim3 grid((unsigned)blocks), block(H::LANES);
+      const dim3 grid((unsigned)blocks), block(lanes);
       if (past) hipLaunchKernelGGL((norm_grad<SPAN, V, J, true, false>), grid, block, 0, stream, P, (int)blocks);
       else hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, false>), grid, block, 0, stream, P, (int)blocks);
     };
