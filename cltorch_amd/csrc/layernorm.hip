@@ -22,8 +22,9 @@ constexpr int kWave = 64;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef f4 f4u __attribute__((aligned(4)));  // a read that only needs the alignment of its elements
 
-// sums of two values over the SPAN threads that share a row, in lane and wave order, for each of them
-template <int SPAN>
+// sums of two values over the SPAN threads that share a row, one of LANES / SPAN rows of the block, in lane and wave
+// order, for each of them
+template <int SPAN, int LANES>
 __device__ __forceinline__ void row_sums(double &a, double &b) {
 #pragma unroll
   for (int d = (SPAN < kWave ? SPAN : kWave) / 2; d > 0; d >>= 1) {
@@ -32,13 +33,14 @@ __device__ __forceinline__ void row_sums(double &a, double &b) {
   }
   if constexpr (SPAN > kWave) {
     constexpr int WAVES = SPAN / kWave;
-    __shared__ double part[2][WAVES];
+    __shared__ double part[2][LANES / kWave];
+    const int first = threadIdx.x / SPAN * WAVES;
     __syncthreads();  // the last sums have been read
     if (threadIdx.x % kWave == 0) part[0][threadIdx.x / kWave] = a, part[1][threadIdx.x / kWave] = b;
     __syncthreads();
-    a = part[0][0], b = part[1][0];
+    a = part[0][first], b = part[1][first];
 #pragma unroll
-    for (int i = 1; i < WAVES; i++) a += part[0][i], b += part[1][i];
+    for (int i = 1; i < WAVES; i++) a += part[0][first + i], b += part[1][first + i];
   }
 }
 
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(SPAN < 256 ? 256 : SPAN) void norm_rows(NormParams 
       if (H::at(j) < width)
 #pragma unroll
         for (int c = 0; c < V; c++) sum += (double)x[V * j + c];
-    row_sums<SPAN>(sum, none);
+    row_sums<SPAN, H::LANES>(sum, none);
     const double mean = sum / (double)width;
     // the mean in two floats: x - mean then loses nothing where the mean is far larger than what varies around it
     const float mh = (float)mean, ml = (float)(mean - (double)mh);
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(SPAN < 256 ? 256 : SPAN) void norm_rows(NormParams 
         x[V * j + c] = d;
         if (H::at(j) < width) squares += (double)d * (double)d;
       }
-    row_sums<SPAN>(squares, none);
+    row_sums<SPAN, H::LANES>(squares, none);
     const float rstd = (float)(1.0 / sqrt(squares / (double)width + (double)P.eps));
 #pragma unroll
     for (int k = 0; k < H::N; k++) x[k] = fmaf(x[k] * rstd, w[k], b[k]);
@@ -221,7 +223,7 @@ __global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, FEW>::LANES)) void no
       if (H::at(k / V) < width) s1 += (double)g, s2 += (double)(g * h[k]);
     }
     if (!P.gx) continue;
-    row_sums<SPAN>(s1, s2);
+    row_sums<SPAN, H::LANES>(s1, s2);
     const float c1 = (float)(s1 * per), c2 = (float)(s2 * per);
 #pragma unroll
     for (int k = 0; k < H::N; k++) h[k] = (gy[k] - c1 - h[k] * c2) * rstd;
@@ -288,7 +290,7 @@ __device__ __forceinline__ void norm_wide_row(const NormParams &P, long row) {
   double s = 0.0, none = 0.0;
 #pragma unroll 4
   for (long i = threadIdx.x; i < P.width; i += kWide) s += (double)x[i];
-  row_sums<kWide>(s, none);
+  row_sums<kWide, kWide>(s, none);
   const double mean = s / (double)P.width;
   const float mh = (float)mean, ml = (float)(mean - (double)mh);
   double q = 0.0;
@@ -297,7 +299,7 @@ __device__ __forceinline__ void norm_wide_row(const NormParams &P, long row) {
     const float d = (x[i] - mh) - ml;
     q += (double)d * (double)d;
   }
-  row_sums<kWide>(q, none);
+  row_sums<kWide, kWide>(q, none);
   const float rstd = (float)(1.0 / sqrt(q / (double)P.width + (double)P.eps));
 #pragma unroll 4
   for (long i = threadIdx.x; i < P.width; i += kWide)
@@ -322,7 +324,7 @@ __device__ __forceinline__ void norm_grad_wide_row(const NormGradParams &P, long
     s1 += (double)g;
     s2 += (double)(g * ((x[i] - mean) * rstd));
   }
-  row_sums<kWide>(s1, s2);
+  row_sums<kWide, kWide>(s1, s2);
   const double per = 1.0 / (double)P.width;
   const float c1 = (float)(s1 * per), c2 = (float)(s2 * per);
 #pragma unroll 4

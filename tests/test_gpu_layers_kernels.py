@@ -228,6 +228,45 @@ def _check_norm_gradient(gx, h, gyw, rstd, what):
     _within(gx, (want, 12 * U * rstd * size), what)
 
 
+@pytest.mark.parametrize("rows,width", [(1100, w) for w in (1, 3, 5, 64, 65, 96, 130, 256, 500, 777, 1000, 1024, 1537, 2048, 3001, 4096, 4099, 6000, 8192, 8195)]
+                         + [(2049, 1537), (3001, 2052), (5003, 24), (2500, 4096)]
+                         + [(16500, 1024), (3000, 8192), (4100, 4099), (20001, 840), (280001, 60), (11000, 1537)])
+def test_layer_norm_of_many_rows(cl, rows, width):
+    """more rows than take part in one launch for all gradients, of every width class, within the caches and past them"""
+    g = _rng("rows", rows, width)
+    x, gy, w, b = _normal(g, rows, width), _normal(g, rows, width), _normal(g, width), _normal(g, width)
+    X, GY, W, B = (cl.ClTensor(a) for a in (x, gy, w, b))
+    y, mean, rstd, gx, gw, gb = (cl.ClTensor() for _ in range(6))
+    y.layerNorm(X, W, B, EPS, mean=mean, rstd=rstd)
+    cl.layerNormBackward(gx, gw, gb, GY, X, W, mean, rstd)
+    x64, g64 = x.astype(np.float64), gy.astype(np.float64)
+    r = 1 / np.sqrt(x64.var(1, keepdims=True) + EPS)
+    h = (x64 - x64.mean(1, keepdims=True)) * r
+    want = h * w + b
+    # x - mean rounds twice, rstd three times, the product and the sum once
+    _within(y.float(), (want, U * (7 * np.abs(h * w) + 2 * np.abs(want)) + 1e-37), "y")
+    # the gradient takes x less the rounded mean, off by up to U |mean| rstd in h
+    eh = 4 * U * np.abs(h) + U * np.abs(x64.mean(1, keepdims=True)) * r
+    gyw = g64 * w
+    c1, c2 = gyw.mean(1, keepdims=True), (gyw * h).mean(1, keepdims=True)
+    size = np.abs(gyw) + np.abs(gyw).mean(1, keepdims=True) + np.abs(h) * np.abs(gyw * h).mean(1, keepdims=True)
+    moved = eh * np.abs(c2) + np.abs(h) * (np.abs(gyw) * eh).mean(1, keepdims=True)
+    _within(gx.float(), (r * (gyw - c1 - h * c2), r * (12 * U * size + moved) + 1e-37), "gx")
+    _within(gw.float(), ((g64 * h).sum(0), (np.abs(g64) * (eh + 2 * U * np.abs(h))).sum(0) + U * np.abs((g64 * h).sum(0)) + 1e-37), "gw")
+    _within(gb.float(), (g64.sum(0), U * np.abs(g64.sum(0)) + 1e-15 * np.abs(g64).sum(0) + 1e-37), "gb")
+    # each by itself, and in place of either operand
+    gx2, gw2, gb2 = cl.ClTensor(), cl.ClTensor(), cl.ClTensor()
+    cl.layerNormBackward(gx2, None, None, GY, X, W, mean, rstd)
+    cl.layerNormBackward(None, gw2, None, GY, X, W, mean, rstd)
+    cl.layerNormBackward(None, None, gb2, GY, X, W, mean, rstd)
+    assert np.array_equal(gx2.float(), gx.float()) and np.array_equal(gw2.float(), gw.float()) and np.array_equal(gb2.float(), gb.float())
+    gw2, gb2 = cl.ClTensor(), cl.ClTensor()
+    cl.layerNormBackward(GY, gw2, gb2, GY, X, W, mean, rstd)
+    assert np.array_equal(GY.float(), gx2.float()) and np.array_equal(gw2.float(), gw.float()) and np.array_equal(gb2.float(), gb.float())
+    X.layerNorm(X, W, B, EPS)
+    assert np.array_equal(X.float(), y.float())
+
+
 def test_layer_norm_of_very_wide_rows(cl):
     """more columns than one launch sums with a block to each 32 of them"""
     width = 33_600_001
