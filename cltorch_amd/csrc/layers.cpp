@@ -287,28 +287,34 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
     if (gradBias) S.gb = thcl_dptr(gradBias), S.gb_step = gradBias->stride[0];
     thcl_slope(state, thcl_ctx(state, THClTensor_getDevice(state, src)), S);
   }
-  Product P;
+  Product P, Q;
   memset(&P, 0, sizeof(P));
+  memset(&Q, 0, sizeof(Q));
+  std::optional<MatrixIn> w;
+  std::optional<RowsIn> x;
+  std::optional<RowsOut> gx, gw;
   if (gradInput) {
-    MatrixIn w(state, weight);
-    RowsOut gx(state, gradInput);
+    w.emplace(state, weight);
+    gx.emplace(state, gradInput);
     P.a = g.p, P.a_m = g.pitch, P.a_k = 1;
-    P.b = w.p, P.b_k = w.s0, P.b_n = w.s1;
-    P.c = gx.p, P.c_m = gx.pitch;
+    P.b = w->p, P.b_k = w->s0, P.b_n = w->s1;
+    P.c = gx->p, P.c_m = gx->pitch;
     P.m = (int)M, P.n = (int)K, P.k = (int)N;
-    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linearBackward");
-    gx.finish();
   }
   if (gradWeight) {
-    RowsIn x(state, src);
-    RowsOut gw(state, gradWeight);
-    P.a = g.p, P.a_m = 1, P.a_k = g.pitch;
-    P.b = x.p, P.b_k = x.pitch, P.b_n = 1;
-    P.c = gw.p, P.c_m = gw.pitch;
-    P.m = (int)N, P.n = (int)K, P.k = (int)M;
-    thcl_product(state, thcl_ctx(state, THClTensor_getDevice(state, src)), P, "linearBackward");
-    gw.finish();
+    x.emplace(state, src);
+    gw.emplace(state, gradWeight);
+    Q.a = g.p, Q.a_m = 1, Q.a_k = g.pitch;
+    Q.b = x->p, Q.b_k = x->pitch, Q.b_n = 1;
+    Q.c = gw->p, Q.c_m = gw->pitch;
+    Q.m = (int)N, Q.n = (int)K, Q.k = (int)M;
   }
+  thcl_rt *rt = thcl_ctx(state, THClTensor_getDevice(state, src));
+  if (gradInput && gradWeight) thcl_product_pair(state, rt, P, Q, "linearBackward");
+  else if (gradInput) thcl_product(state, rt, P, "linearBackward");
+  else if (gradWeight) thcl_product(state, rt, Q, "linearBackward");
+  if (gx) gx->finish();
+  if (gw) gw->finish();
   THCL_GUARD_END()
 }
 

@@ -49,9 +49,18 @@ struct Product {
 // 64 of them in a tile
 struct ThclProductPlan {
   int kind, blocks, most_sharers, slices;
+  double us;  // what it is expected to take
 };
 ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus);
 void thcl_product(THClState *state, thcl_rt *rt, const Product &P, const char *what);
+
+// A linear layer's gradients by its input, P, and its weight, Q, neither ragged: in one launch where that is faster
+// (kind as above; 0: in two).
+struct ThclPairPlan {
+  int kind, slices_p, slices_q;
+};
+ThclPairPlan thcl_pair_plan(const Product &P, const Product &Q, int cus);
+void thcl_product_pair(THClState *state, thcl_rt *rt, const Product &P, const Product &Q, const char *what);
 
 // gz = gy act'(z) and the sums of its columns; gz or gb is NULL when it is not wanted
 struct SlopeParams {

@@ -440,6 +440,10 @@ struct Tile {
   static constexpr int SIMD = SIMD_;  // waves that have to fit a SIMD's registers
   static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
 };
+typedef Tile<256, 256, 2, 4, 7, 2> Tile256;
+typedef Tile<128, 128, 2, 4, 4, 4> Tile128;
+typedef Tile<64, 128, 2, 2, 4, 3> Tile64;
+typedef Tile<32, 128, 1, 4, 2, 4> Tile32;
 
 // Blocks go to the 8 XCDs in turn, and each XCD has its own L2: its blocks get neighbouring numbers.
 __device__ __forceinline__ int numbered_by_xcd(int id, int total) { return id % 8 * (total / 8) + min(id % 8, total % 8) + id / 8; }
@@ -495,21 +499,23 @@ __device__ __forceinline__ float *part_of(const Product &P, const Sharing &h, lo
 
 // RUNS: the ragged products, whose tiles the host cannot count; others have a block to each tile and slice of k, which
 // starts sooner (1000 x 64 x 64: 6.6 us against 8.0) and leaves whole rows of partial results.
+template <class T>
+struct Slabs {  // two arrays, so that the compiler knows that the slab being written is not the one being read
+  static constexpr int BYTES = Staged<T::BM, T::MT>::BYTES + Staged<T::BN, T::NT>::BYTES;
+};
 template <class T, bool AKC, bool BKC, bool RUNS>
-__global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
+__device__ __forceinline__ void split_block(const Product &P, int block, int blocks, int slice, char *lds0, char *lds1) {
   constexpr int MT = T::MT, NT = T::NT;
   typedef Feed<T::BM, MT, AKC, T::TH> FA;
   typedef Feed<T::BN, NT, BKC, T::TH> FB;
   typedef Staged<T::BM, MT> SA;
   typedef Staged<T::BN, NT> SB;
-  // two arrays, so that the compiler knows that the slab being written is not the one being read
-  __shared__ __attribute__((aligned(16))) char lds0[SA::BYTES + SB::BYTES], lds1[SA::BYTES + SB::BYTES];
   const int wave = uniform((int)threadIdx.x / kWave), lane = threadIdx.x % kWave;
-  const int blocks = gridDim.x, me = numbered_by_xcd(blockIdx.x, blocks);
+  const int me = numbered_by_xcd(block, blocks);
   Sharing h;
   long u = 0, u_end = 0;
   if (RUNS) {
-    if (!share_out<T::BM, T::BN, T::START>(P, blocks, blockIdx.x == 0, h)) return;
+    if (!share_out<T::BM, T::BN, T::START>(P, blocks, block == 0, h)) return;
     u = uniform(me * h.run);
     u_end = uniform(P.ragged == DEPTH ? u + h.run : min(u + h.run, h.shared * (h.slabs + T::START)));
   } else {
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
     }
     if (!RUNS) {  // this block's slice of k
       const int per = (slabs + P.slices - 1) / P.slices;
-      s0 = min((int)blockIdx.z * per, slabs);
+      s0 = min(slice * per, slabs);
       n = min(per, slabs - s0);
     }
     if (!RUNS || P.ragged != DEPTH) {
@@ -689,7 +695,7 @@ __global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
     // partial results: a tile by rows, or, in slices, the whole matrix
     float *part = nullptr;
     if (RUNS && n < slabs) part = part_of(P, h, me, unit0, T::BM * T::BN) - (long)w.row0 * T::BN - col0 + col;
-    if (!RUNS && P.slices > 1) part = P.work + (long)blockIdx.z * P.m * P.n + col;
+    if (!RUNS && P.slices > 1) part = P.work + (long)slice * P.m * P.n + col;
     const long part_pitch = RUNS ? T::BN : P.n;
     if (inside) {
 #pragma unroll
@@ -718,6 +724,22 @@ __global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
       }
     }
   }
+}
+
+template <class T, bool AKC, bool BKC, bool RUNS>
+__global__ __launch_bounds__(T::TH, T::SIMD) void product_split(Product P) {
+  __shared__ __attribute__((aligned(16))) char lds0[Slabs<T>::BYTES], lds1[Slabs<T>::BYTES];
+  split_block<T, AKC, BKC, RUNS>(P, blockIdx.x, gridDim.x, blockIdx.z, lds0, lds1);
+}
+
+// The two products of a linear layer's gradient, gz W and gz^T x, in one launch, a tile and slice of k to a block: where
+// neither fills the chip by itself.
+template <class T>
+__global__ __launch_bounds__(T::TH, T::SIMD) void product_pair(Product P, Product Q, int tiles_p, int tiles_q) {
+  __shared__ __attribute__((aligned(16))) char lds0[Slabs<T>::BYTES], lds1[Slabs<T>::BYTES];
+  const int id = blockIdx.x - tiles_p * P.slices;
+  if (id < 0) split_block<T, true, false, false>(P, blockIdx.x % tiles_p, tiles_p, blockIdx.x / tiles_p, lds0, lds1);
+  else split_block<T, false, false, false>(Q, id % tiles_q, tiles_q, id / tiles_q, lds0, lds1);
 }
 
 // The parts of the shared tiles, added in the order of k, and the epilogue: a block takes 16 rows of a tile
@@ -983,7 +1005,7 @@ __global__ __launch_bounds__(64 * kThinWaves, 2) void product_thin(Product P) {
 
 // The slices of k of every result, added in order, and the epilogue: a block takes 256 columns of 8 rows, walking down.
 constexpr int kSliceRows = 8;
-__global__ __launch_bounds__(256) void add_slices(Product P) {
+__device__ __forceinline__ void add_slices_of(const Product &P, int block, int blocks) {
   int rows = P.m;
   if (P.ragged == ROWS) {
     const Totals t = count_groups(P.sizes, P.groups, P.m, Units{0, 0, 0});
@@ -994,7 +1016,7 @@ __global__ __launch_bounds__(256) void add_slices(Product P) {
   if (col >= P.n) return;
   const Column line(P, col);
   const long per = (long)P.m * P.n;
-  for (long row = (long)blockIdx.y * kSliceRows; row < rows; row += (long)gridDim.y * kSliceRows) {
+  for (long row = (long)block * kSliceRows; row < rows; row += (long)blocks * kSliceRows) {
     float sum[kSliceRows];
 #pragma unroll
     for (int i = 0; i < kSliceRows; i++) sum[i] = 0.f;
@@ -1005,6 +1027,12 @@ __global__ __launch_bounds__(256) void add_slices(Product P) {
     }
     line.finish_rows<kSliceRows>(P, P.c, (int)row, 1, rows, sum);
   }
+}
+
+__global__ __launch_bounds__(256) void add_slices(Product P) { add_slices_of(P, blockIdx.y, gridDim.y); }
+__global__ __launch_bounds__(256) void add_slices_pair(Product P, Product Q, int blocks_p) {
+  if ((int)blockIdx.y < blocks_p) add_slices_of(P, blockIdx.y, blocks_p);
+  else add_slices_of(Q, blockIdx.y - blocks_p, gridDim.y - blocks_p);
 }
 
 // gz = gy act'(z), and the sums of its columns: a block takes 256 columns of a run of rows and leaves its part of the
@@ -1078,6 +1106,10 @@ namespace {
 struct TileCost {
   int bm, bn, resident;
   double alone, full, start;
+  double busy(double per) const {  // a block's time per slab with `per` blocks to a compute unit
+    if (per <= 1) return resident > 1 ? alone : alone + (full - alone) * per;
+    return alone + (full - alone) * (per - 1) / (resident - 1);
+  }
 };
 constexpr TileCost kTiles[4] = {{256, 256, 1, 1.51, 2.07, 7.8}, {128, 128, 2, 0.62, 1.28, 4.0}, {64, 128, 3, 0.51, 1.14, 4.1}, {32, 128, 4, 0.43, 1.11, 2.2}};
 struct ThinCost {
@@ -1090,10 +1122,10 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
   const int groups = P.groups < P.m ? P.groups : P.m;  // that can hold rows
   const double share = 256. / cus;
   const double k = P.ragged == DEPTH ? (double)P.k / P.groups : P.k, outputs = (double)P.m * P.n;
-  ThclProductPlan best{0, 1, 1, 1};
+  ThclProductPlan best{0, 1, 1, 1, INFINITY};
   double least = INFINITY;
   auto consider = [&](const ThclProductPlan &plan, double us) {
-    if (us < least) least = us, best = plan;
+    if (us < least) least = us, best = plan, best.us = us;
   };
   // row tiles of a ragged product, on the average over where groups end
   auto row_tiles = [&](int rows) {
@@ -1104,10 +1136,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
     const TileCost &c = kTiles[t];
     const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
     const double slabs = std::fmax(std::ceil(k / KS), 1.), stream = 4. * ((double)P.m * P.k + (double)P.k * P.n + outputs) / 3500e3 * share;
-    auto busy = [&](double per) {  // a block's time per slab with `per` blocks to a compute unit
-      if (per <= 1) return c.resident > 1 ? c.alone : c.alone + (c.full - c.alone) * per;
-      return c.alone + (c.full - c.alone) * (per - 1) / (c.resident - 1);
-    };
+    auto busy = [&](double per) { return c.busy(per); };
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {  // blocks to a tile
       if (s > 1 && slabs / s < 4) break;
       if (P.ragged == WHOLE) {
@@ -1117,7 +1146,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
         double us = 4.4 + (turns * busy(c.resident) + (rest > 0 ? busy(rest) : 0.)) * (std::ceil(slabs / s) + c.start);
         us = std::fmax(us, 4.4 + stream);
         if (s > 1) us += 4.8 + 4. * outputs * (2 * s + 1) / 14700e3;
-        consider(ThclProductPlan{t, 1, 1, s}, us);
+        consider(ThclProductPlan{t, 1, 1, s, us}, us);
       } else {
         const int blocks = (int)std::fmin((double)cus * c.resident, std::ceil(tiles) * s);
         const double rounds = P.ragged == DEPTH ? 0. : std::floor(tiles / blocks), shared = tiles - rounds * blocks;
@@ -1126,7 +1155,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
         if (shared > 0) us += busy(std::ceil(sharers * share / 256.)) * run;
         // the parts are written and read, the tiles written
         if (P.ragged == DEPTH || s > 1) us += 4.8 + 4. * c.bm * c.bn * (2 * sharers + shared) / 13800e3;
-        consider(ThclProductPlan{t, blocks, s, 1}, us);
+        consider(ThclProductPlan{t, blocks, s, 1, us}, us);
       }
     }
   }
@@ -1140,9 +1169,38 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
       for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (s > 1 && (k < 2 * kThinStep * kThinWaves * s || s * outputs * 4 > 1e9)) break;
         const double rate = std::fmin(tiles * s * c.alone, c.chip / share);
-        consider(ThclProductPlan{4 + mt - 1, 1, 1, s}, 4.5 + bytes / rate / 1e3 + (s > 1 ? 4.8 + 4. * outputs * (2 * s + 1) / 14700e3 : 0.));
+        consider(ThclProductPlan{4 + mt - 1, 1, 1, s, 0.}, 4.5 + bytes / rate / 1e3 + (s > 1 ? 4.8 + 4. * outputs * (2 * s + 1) / 14700e3 : 0.));
       }
     }
+  }
+  return best;
+}
+
+// Two products in one launch of equal tiles, each with its own slices of k; kind 0 where two launches are as good.  Both
+// together fill the chip where one does not and need one launch to add their slices: gradients of 300 x 300 x 300 22.8 ->
+// 12.8 us, 628 x 820 x 1224 48 -> 33, 1000^3 52 -> 40, 3000 x 700 x 900 89 -> 77; from 2048^3 on they take two.
+ThclPairPlan thcl_pair_plan(const Product &P, const Product &Q, int cus) {
+  ThclPairPlan best{0, 1, 1};
+  double least = thcl_product_plan(P, false, cus).us + thcl_product_plan(Q, false, cus).us;
+  const double share = 256. / cus;
+  constexpr int N = 8, cuts[N] = {1, 2, 3, 4, 6, 8, 12, 16};
+  const long slabs_p = (P.k - 1) / KS + 1, slabs_q = (Q.k - 1) / KS + 1;
+  for (int t = 1; t < 4; t++) {
+    const TileCost &c = kTiles[t];
+    auto tiles = [&](const Product &X) { return (double)((X.m - 1) / c.bm + 1) * ((X.n - 1) / c.bn + 1); };
+    const double tiles_p = tiles(P), tiles_q = tiles(Q);
+    for (int i = 0; i < N && (i == 0 || slabs_p >= 4 * cuts[i]); i++)
+      for (int j = 0; j < N && (j == 0 || slabs_q >= 4 * cuts[j]); j++) {
+        const int sp = cuts[i], sq = cuts[j];
+        const double np = (slabs_p - 1) / sp + 1 + c.start, nq = (slabs_q - 1) / sq + 1 + c.start, longest = np > nq ? np : nq;
+        const double blocks = tiles_p * sp + tiles_q * sq;
+        const double bytes = 4. * ((sp > 1 ? 2 * sp + 1 : 0) * (double)P.m * P.n + (sq > 1 ? 2 * sq + 1 : 0) * (double)Q.m * Q.n);
+        if (bytes > 1e9 || blocks > 1e6) continue;
+        const double per = blocks * share / 256., all = (tiles_p * sp * np + tiles_q * sq * nq) * share / 256.;
+        double us = 4.4 + (per <= c.resident ? c.busy(std::ceil(per)) * longest : c.full / c.resident * (all + 0.5 * longest));
+        if (sp > 1 || sq > 1) us += 4.8 + bytes / 14700e3;
+        if (us < least) least = us, best = ThclPairPlan{t, sp, sq};
+      }
   }
   return best;
 }
@@ -1209,10 +1267,10 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
     THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
   }
   switch (plan.kind) {
-    case 0: launch_split<Tile<256, 256, 2, 4, 7, 2>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 1: launch_split<Tile<128, 128, 2, 4, 4, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 2: launch_split<Tile<64, 128, 2, 2, 4, 3>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
-    case 3: launch_split<Tile<32, 128, 1, 4, 2, 4>>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 0: launch_split<Tile256>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 1: launch_split<Tile128>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 2: launch_split<Tile64>(P, akc, bkc && akc, plan.blocks, stream, what); break;
+    case 3: launch_split<Tile32>(P, akc, bkc && akc, plan.blocks, stream, what); break;
     case 4: launch_thin<1>(P, bkc, row_tiles(16), stream, what); break;
     case 5: launch_thin<2>(P, bkc, row_tiles(32), stream, what); break;
     case 6: launch_thin<3>(P, bkc, row_tiles(48), stream, what); break;
@@ -1221,6 +1279,48 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
   if (P.slices > 1) {
     const int down = (P.m - 1) / kSliceRows + 1;
     hipLaunchKernelGGL(add_slices, dim3((unsigned)((P.n - 1) / 256 + 1), (unsigned)(down < 65535 ? down : 65535)), dim3(256), 0, stream, P);
+    check_launch(what);
+  }
+  thcl_after_launch(state, rt);
+}
+
+template <class T>
+static void launch_pair(const Product &P, const Product &Q, hipStream_t stream) {
+  auto tiles = [](const Product &X) { return ((X.m - 1) / T::BM + 1) * ((X.n - 1) / T::BN + 1); };
+  const int p = tiles(P), q = tiles(Q);
+  hipLaunchKernelGGL((product_pair<T>), dim3(p * P.slices + q * Q.slices), dim3(T::TH), 0, stream, P, Q, p, q);
+}
+
+void thcl_product_pair(THClState *state, thcl_rt *rt, const Product &first, const Product &second, const char *what) {
+  Product P = first, Q = second;
+  ThclPairPlan plan{0, 1, 1};
+  const bool fits = P.a_k == 1 && P.b_n == 1 && Q.a_m == 1 && Q.b_n == 1 && P.a_m < kFarPitch && P.b_k < kFarPitch && Q.a_k < kFarPitch && Q.b_k < kFarPitch;
+  if (fits && P.m > 64) plan = thcl_pair_plan(P, Q, thcl_rt_get_props(rt)->compute_units);
+  if (plan.kind == 0) {
+    thcl_product(state, rt, P, what);
+    thcl_product(state, rt, Q, what);
+    return;
+  }
+  hipStream_t stream = (hipStream_t)thcl_rt_stream(rt);
+  P.slices = plan.slices_p;
+  Q.slices = plan.slices_q;
+  const size_t floats_p = P.slices > 1 ? (size_t)P.slices * P.m * P.n : 0, floats_q = Q.slices > 1 ? (size_t)Q.slices * Q.m * Q.n : 0;
+  if (floats_p + floats_q) {
+    P.work = (float *)thcl_rt_workspace(rt, (floats_p + floats_q) * sizeof(float));
+    THCL_CHECK(P.work != nullptr, "%s workspace: %s", what, thcl_rt_error());
+    Q.work = P.work + floats_p;
+  }
+  switch (plan.kind) {
+    case 1: launch_pair<Tile128>(P, Q, stream); break;
+    case 2: launch_pair<Tile64>(P, Q, stream); break;
+    default: launch_pair<Tile32>(P, Q, stream); break;
+  }
+  check_launch(what);
+  auto down = [](const Product &X) { return X.slices > 1 ? (X.m - 1) / kSliceRows + 1 : 0; };
+  const int p = down(P) < 32767 ? down(P) : 32767, q = down(Q) < 32767 ? down(Q) : 32767;
+  if (p + q) {
+    const int n = p == 0 ? Q.n : q == 0 ? P.n : P.n > Q.n ? P.n : Q.n;
+    hipLaunchKernelGGL(add_slices_pair, dim3((unsigned)((n - 1) / 256 + 1), (unsigned)(p + q)), dim3(256), 0, stream, P, Q, p);
     check_launch(what);
   }
   thcl_after_launch(state, rt);

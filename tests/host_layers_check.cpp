@@ -89,6 +89,10 @@ void thcl_product(THClState *, thcl_rt *, const Product &P, const char *) {
       }
   }
 }
+void thcl_product_pair(THClState *state, thcl_rt *rt, const Product &P, const Product &Q, const char *what) {
+  thcl_product(state, rt, P, what);
+  thcl_product(state, rt, Q, what);
+}
 void thcl_slope(THClState *, thcl_rt *, const SlopeParams &P) {
   g_launches++;
   for (long i = 0; i < P.width; i++) {
@@ -102,7 +106,6 @@ void thcl_slope(THClState *, thcl_rt *, const SlopeParams &P) {
     if (P.gb) P.gb[i * P.gb_step] = (float)sum;
   }
 }
-ThclProductPlan thcl_product_plan(const Product &, bool, int) { return {0, 0, 0, 0}; }
 
 // ---- views ------------------------------------------------------------------------------------------------------
 static THClState *S;

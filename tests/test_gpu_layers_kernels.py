@@ -48,10 +48,43 @@ def test_linear_in_every_tile(cl, rows, inner, outer):
     _within(got, (relu + gy, tol + U * np.abs(want + b) + U * np.abs(relu + gy)), "y")
     y.linear(X, W, cl.ClTensor(b), residual=GY, activation="relu", preact=pre)
     assert np.array_equal(y.float().view(np.uint32), got.view(np.uint32))  # the order of sums does not change
-    gx, gw = cl.ClTensor(), cl.ClTensor()
+    gx, gw, gx1, gw1 = (cl.ClTensor() for _ in range(4))
     cl.linearBackward(gx, gw, None, GY, X, W)
-    _within(gx.float(), _product(gy, w), "gx")
-    _within(gw.float(), _product(gy.T, x), "gw")
+    cl.linearBackward(gx1, None, None, GY, X, W)
+    cl.linearBackward(None, gw1, None, GY, X, W)
+    want = _product(gy, w)
+    _within(gx.float(), want, "gx")
+    _within(gx1.float(), want, "gx alone")
+    want = _product(gy.T, x)
+    _within(gw.float(), want, "gw")
+    _within(gw1.float(), want, "gw alone")
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(150, 300, 260), (628, 820, 1224), (70, 600, 70)])
+def test_gradients_together_with_infinities_and_tiny_values(cl, rows, inner, outer):
+    """what does not split keeps to its rows and columns of either gradient where both come from one launch"""
+    g = _rng("pair", rows, inner, outer)
+    x, w, gy = _normal(g, rows, inner), _normal(g, outer, inner), _normal(g, rows, outer)
+    gy[3, 5], x[7, 11], w[9, 2] = np.inf, np.nan, -np.inf
+    gx, gw = cl.ClTensor(), cl.ClTensor()
+    cl.linearBackward(gx, gw, None, cl.ClTensor(gy), cl.ClTensor(x), cl.ClTensor(w))
+    for got, a, b in ((gx.float(), gy, w), (gw.float(), gy.T, x)):
+        with np.errstate(invalid="ignore"):
+            want = a.astype(np.float64) @ b
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want)) and np.array_equal(np.isneginf(got), np.isneginf(want))
+        fine = np.isfinite(want)
+        tol = _product(np.where(np.isfinite(a), a, 0), np.where(np.isfinite(b), b, 0))[1]
+        _within(np.where(fine, got, 0), (np.where(fine, want, 0), tol), "beside infinities")
+    x, w, gy = _normal(g, rows, inner), _normal(g, outer, inner), _normal(g, rows, outer)
+    gy[2] = np.clip(gy[2], -3, 3) * F(1e-37)
+    gy[2][np.abs(gy[2]) < 1.2e-38] = 0
+    w[:, 4] = np.clip(w[:, 4], -3, 3) * F(1e36)
+    cl.linearBackward(gx, gw, None, cl.ClTensor(gy), cl.ClTensor(x), cl.ClTensor(w))
+    # 1e-38 per term: products and sums below the normal range may round to its grid or to zero
+    want, tol = _product(gy, w)
+    _within(gx.float(), (want, tol + outer * 1.2e-38), "gx")
+    want, tol = _product(gy.T, x)
+    _within(gw.float(), (want, tol + rows * 1.2e-38), "gw")
 
 
 @pytest.mark.parametrize("rows,inner,outer,sizes", GROUPED)

@@ -117,5 +117,14 @@ void thcl_dbg_product_plan(int ragged, int m, int n, int k, int groups, int few_
   const ThclProductPlan got = thcl_product_plan(P, few_rows_fit != 0, cus);
   plan[0] = got.kind, plan[1] = got.blocks, plan[2] = got.most_sharers, plan[3] = got.slices;
 }
+
+// the gradients of a linear layer together; plan: kind, slices of the input's, slices of the weight's
+void thcl_dbg_pair_plan(int rows, int inner, int outer, int cus, int *plan) {
+  Product P = {}, Q = {};
+  P.m = rows, P.n = inner, P.k = outer;
+  Q.m = outer, Q.n = inner, Q.k = rows;
+  const ThclPairPlan got = thcl_pair_plan(P, Q, cus);
+  plan[0] = got.kind, plan[1] = got.slices_p, plan[2] = got.slices_q;
+}
 #endif
 }

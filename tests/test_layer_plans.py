@@ -61,6 +61,31 @@ def test_every_choice_can_be_launched(hooks_lib, cus):
                             assert 1 <= blocks <= cus * TILES[kind][2] and slices == 1
 
 
+def _pair(lib, rows, inner, outer, cus=256):
+    p = (C.c_int * 3)()
+    lib.thcl_dbg_pair_plan(rows, inner, outer, cus, p)
+    return tuple(p)
+
+
+def test_gradients_share_a_launch(hooks_lib):
+    """the tested shapes take two launches and each tile of one, with either product split and whole"""
+    plans = [_pair(hooks_lib, *shape) for shape in LINEAR if shape[0] > 64]
+    assert {kind for kind, _, _ in plans} == {0, 1, 2, 3}, plans
+    shared = {(p > 1, q > 1) for kind, p, q in plans if kind}
+    assert shared == {(False, False), (False, True), (True, False), (True, True)}, plans
+    for cus in (256, 64, 1):
+        for rows in (65, 1000, 40000, 2 ** 31 - 70000):
+            for inner in (1, 130, 5000, 2 ** 31 - 70000):
+                for outer in (1, 500, 2 ** 20, 2 ** 31 - 70000):
+                    kind, p, q = _pair(hooks_lib, rows, inner, outer, cus)
+                    if not kind:
+                        continue
+                    bm, bn, _ = TILES[kind]
+                    blocks = -(-rows // bm) * -(-inner // bn) * p + -(-outer // bm) * -(-inner // bn) * q
+                    assert blocks <= 1e6 and 4 * (p * rows * inner * (p > 1) + q * outer * inner * (q > 1)) <= 1e9
+                    assert (p == 1 or -(-outer // 16) >= 4 * p) and (q == 1 or -(-rows // 16) >= 4 * q)
+
+
 def test_few_rows_only_where_they_fit(hooks_lib):
     for m in (1, 16, 64):
         assert _plan(hooks_lib, WHOLE, m, 4096, 4096, few=False)[0] < 4
