@@ -1099,7 +1099,7 @@ void check_launch(const char *what) {
 //                 of one, 68 us against 50 and 60 for 1531 x 1027 x 2053
 //   start         what a block's first loads and its epilogue cost, in slabs
 //   stream        the operands' bytes, of which the tiles get 3.5 TB/s
-//   adding        the launch that adds the parts of shared tiles costs 4.8 us and its bytes
+//   adding        the launch that adds slices or the parts of shared tiles costs 4.8 or 7.4 us and its bytes
 // Up to 64 rows the kernel for few rows takes part, with what a block of 16 to 64 rows reads per nanosecond (`alone`)
 // and what the chip reaches (1 x 4096 x 16384: 46 us, in tiles 64).
 namespace {
@@ -1112,6 +1112,9 @@ struct TileCost {
   }
 };
 constexpr TileCost kTiles[4] = {{256, 256, 1, 1.51, 2.07, 7.8}, {128, 128, 2, 0.62, 1.28, 4.0}, {64, 128, 3, 0.51, 1.14, 4.1}, {32, 128, 4, 0.43, 1.11, 2.2}};
+// the ragged products, fitted to 12 shapes with groups of random sizes, 2 % over the best choice
+constexpr TileCost kRowTiles[4] = {{256, 256, 1, 1.48, 2.14, 7.8}, {128, 128, 2, 0.81, 1.43, 4.8}, {64, 128, 3, 0.55, 1.21, 3.6}, {32, 128, 4, 0.45, 1.31, 2.0}};
+constexpr TileCost kDepthTiles[4] = {{256, 256, 1, 1.20, 2.80, 6.7}, {128, 128, 2, 1.26, 1.91, 4.4}, {64, 128, 3, 0.84, 1.54, 4.4}, {32, 128, 4, 0.73, 1.55, 2.7}};
 struct ThinCost {
   double alone, chip;  // bytes per nanosecond
 };
@@ -1127,13 +1130,13 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
   auto consider = [&](const ThclProductPlan &plan, double us) {
     if (us < least) least = us, best = plan, best.us = us;
   };
-  // row tiles of a ragged product, on the average over where groups end
+  // row tiles; of groups of random sizes, whose rows are taken to be distributed exponentially
   auto row_tiles = [&](int rows) {
     if (P.ragged != ROWS) return (double)((P.m + rows - 1) / rows);
-    return P.m <= (double)rows * groups ? (double)groups : (double)P.m / rows + 0.5 * groups;
+    return groups / (1. - std::exp(-(double)rows * groups / P.m));
   };
   for (int t = 0; t < 4; t++) {
-    const TileCost &c = kTiles[t];
+    const TileCost &c = P.ragged == WHOLE ? kTiles[t] : P.ragged == ROWS ? kRowTiles[t] : kDepthTiles[t];
     const double tiles = row_tiles(c.bm) * ((P.n + c.bn - 1) / c.bn) * (P.ragged == DEPTH ? P.groups : 1);
     const double slabs = std::fmax(std::ceil(k / KS), 1.), stream = 4. * ((double)P.m * P.k + (double)P.k * P.n + outputs) / 3500e3 * share;
     auto busy = [&](double per) { return c.busy(per); };
@@ -1151,10 +1154,10 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
         const int blocks = (int)std::fmin((double)cus * c.resident, std::ceil(tiles) * s);
         const double rounds = P.ragged == DEPTH ? 0. : std::floor(tiles / blocks), shared = tiles - rounds * blocks;
         const double sharers = std::fmin(blocks, shared * s), run = std::ceil(shared * (slabs + c.start) / sharers);
-        double us = 5.5 + rounds * busy(std::ceil(blocks * share / 256.)) * (slabs + c.start);
+        double us = 8.0 + rounds * busy(std::ceil(blocks * share / 256.)) * (slabs + c.start);
         if (shared > 0) us += busy(std::ceil(sharers * share / 256.)) * run;
         // the parts are written and read, the tiles written
-        if (P.ragged == DEPTH || s > 1) us += 4.8 + 4. * c.bm * c.bn * (2 * sharers + shared) / 13800e3;
+        if (P.ragged == DEPTH || s > 1) us += 7.4 + 4. * c.bm * c.bn * (2 * sharers + shared) / 7600e3;
         consider(ThclProductPlan{t, blocks, s, 1, us}, us);
       }
     }
@@ -1165,7 +1168,8 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
     const int mt = (int)std::ceil(rows * (P.ragged == ROWS ? 1.5 : 1.) / 16);
     if (mt >= 1 && mt <= 4) {
       const ThinCost &c = kThin[mt - 1];
-      const double tiles = row_tiles(16 * mt) * ((P.n + kThinCols - 1) / kThinCols), bytes = 4. * P.k * P.n * row_tiles(16 * mt);
+      // groups that take two tiles find b in the caches for the second one
+      const double matrices = P.ragged == ROWS ? groups : 1, tiles = matrices * ((P.n + kThinCols - 1) / kThinCols), bytes = 4. * P.k * P.n * matrices;
       for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (s > 1 && (k < 2 * kThinStep * kThinWaves * s || s * outputs * 4 > 1e9)) break;
         const double rate = std::fmin(tiles * s * c.alone, c.chip / share);
