@@ -462,7 +462,7 @@ __device__ __forceinline__ void tile_of(long tile, int tiles_m, int tiles_n, int
 // finishes the tile.  (Added by the block that comes last, in the same launch, they cost more: one compute unit reads
 // some 17 bytes per nanosecond, and 1024^3 in 128 x 128 tiles took 59 us against 29.)
 // A tile counts as START slabs more than it has, its first loads and its epilogue: the blocks that got the tiles of small
-// groups would else be the last by far (weights' gradient of 4095 rows in 8 groups of 45 to 1200: 274 us).
+// groups would else be the last by far (weights' gradient of 4095 rows in 8 groups of 45 to 1200: 274 us against 157).
 struct Sharing {
   int tiles_m, tiles_n, slabs;  // DEPTH: slabs is by group
   int rounds;

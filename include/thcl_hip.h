@@ -569,9 +569,9 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
                                THClTensor *gradOutput, THClTensor *src, THClTensor *weight, THClTensor *preact,
                                int activation);
 /* Rows of src [rows, in] lie group after group, sizes[g] of them each: every row is multiplied by its group's matrix
- * of weight [groups, in, out] (up to 65535 groups).  sizes is a vector of whole numbers as floats (below 2^24 each).  Rows behind the last
- * group are left as they were.  Sizes that are negative, no whole numbers or come to more than the rows make the call
- * write nothing; the next call that waits for the stream reports it, as for an index out of range. */
+ * of weight [groups, in, out] (up to 65535 groups).  sizes is a vector of whole numbers as floats (below 2^24 each).
+ * Rows behind the last group are left as they were.  Sizes that are negative, no whole numbers or come to more than the
+ * rows make the call write nothing; the next call that waits for the stream reports it, as for an index out of range. */
 void THClTensor_groupedmm(THClState *state, THClTensor *self, THClTensor *src, THClTensor *weight, THClTensor *sizes);
 /* Gradients by src (rows behind the last group are left as they were) and by weight (zero for a group without rows),
  * each or NULL. */
