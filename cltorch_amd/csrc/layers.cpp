@@ -326,10 +326,10 @@ void THClTensor_groupedmm(THClState *state, THClTensor *self, THClTensor *src, T
   const long T = src->size[0], K = src->size[1], G = weight->size[0], N = weight->size[2];
   THCL_ARGCHECK(weight->size[1] == K, 4, "a group's matrix must have a row per input feature");
   THCL_ARGCHECK(sizes->nDimension == 1 && sizes->size[0] == G, 5, "vector with the rows of each group expected");
+  THCL_ARGCHECK(G <= 65535, 4, "at most 65535 groups expected");
   check_int(T);
   check_int(N);
   check_int(K);
-  check_int(G);
   Shape shape = shape2(T, N);
   THClTensor *operands[3] = {src, weight, sizes};
   for (int o = 0; o < 3; o++) thcl_check_apart(self, shape, operands[o], false, "the result");
@@ -371,10 +371,10 @@ void THClTensor_groupedmmBackward(THClState *state, THClTensor *gradInput, THClT
   THCL_ARGCHECK(weight->size[1] == K, 6, "a group's matrix must have a row per input feature");
   THCL_ARGCHECK(gradOutput->nDimension == 2 && gradOutput->size[0] == T && gradOutput->size[1] == N, 4, "gradOutput must have the result's shape");
   THCL_ARGCHECK(sizes->nDimension == 1 && sizes->size[0] == G, 7, "vector with the rows of each group expected");
+  THCL_ARGCHECK(G <= 65535, 6, "at most 65535 groups expected");
   check_int(T);
   check_int(N);
   check_int(K);
-  check_int(G);
   Shape w_shape(weight);
   const Shape in(src);
   THClTensor *results[2] = {gradInput, gradWeight}, *operands[4] = {gradOutput, src, weight, sizes};

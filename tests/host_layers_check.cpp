@@ -354,6 +354,10 @@ static void refusals() {
   NO(THClTensor_groupedmm(S, y.t, v8.t, w3.t, s2.t));
   NO(THClTensor_groupedmm(S, x.t, x.t, w3.t, s2.t));
   NO(THClTensor_groupedmmBackward(S, x2.t, nullptr, x.t, x.t, w3.t, s2.t));
+  T many = view({65536, 8, 5}, 3), sizes = view({65536}, 3);
+  NO(THClTensor_groupedmm(S, y.t, x.t, many.t, sizes.t));
+  NO(THClTensor_groupedmmBackward(S, x2.t, nullptr, y.t, x.t, many.t, sizes.t));
+  NO(THClTensor_groupedmm(S, s2.t, x.t, w3.t, s2.t));
   NO(THClTensor_groupedmmBackward(S, x2.t, w3.t, y.t, x.t, w3.t, s2.t));
   NO(THClTensor_groupedmmBackward(S, y.t, nullptr, y.t, x.t, w3.t, s2.t));
   // memory shared at other places than the same ones; a result that repeats its elements
