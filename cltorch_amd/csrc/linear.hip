@@ -35,11 +35,17 @@ __device__ __forceinline__ float exp2_sum(float h, float l) {
   const float e = __builtin_amdgcn_exp2f(h);
   return fmaf(e, l * kLn2, e);
 }
-__device__ __forceinline__ float sigmoid(float z) {
-  const float h = -z * kLog2e, l = fmaf(-z, kLog2e, -h) - z * kLog2eRest;
-  // up to 2^120: beyond, one more than it is no more than it, and its reciprocal is nothing beside any z
-  return reciprocal(1.f + exp2_sum(fminf(h, 120.f), h < 120.f ? l : 0.f));
-}
+// 1 / (1 + e) and e = exp(-|z|), which is held 2^64 too large where it would leave the normal numbers; 0 far beyond that
+struct Logistic {
+  float near, e, scale;  // sigmoid(|z|); exp(-|z|) is e scale
+  __device__ __forceinline__ explicit Logistic(float z) {
+    const float a = fminf(fabsf(z), 128.f), h = -a * kLog2e, l = fmaf(-a, kLog2e, -h) - a * kLog2eRest;
+    const bool far = a > 80.f;
+    e = exp2_sum(far ? h + 64.f : h, l);
+    scale = far ? 0x1p-64f : 1.f;
+    near = reciprocal(1.f + e * scale);
+  }
+};
 // The part of the normal distribution beyond |z| on both sides, erfc(x) with x = |z| / sqrt(2), and exp(-x^2).  With
 // t = 3 / (3 + x), erfc(x) exp(x^2) / t is a polynomial of degree 9 in t to 8e-9 of its value, fitted to erfcx over x up
 // to 14.2; x^2 is taken in two floats, so the tail keeps its digits.
@@ -71,10 +77,16 @@ __device__ __forceinline__ float gelu_slope(float z) {
   const float half = 0.5f * two_tails(fminf(fabsf(z), 20.f), gauss);
   return z != z ? z : fmaf(fmaxf(fminf(z, 20.f), -20.f) * 0.3989422804014327f, gauss, z > 0.f ? 1.f - half : half);
 }
-__device__ __forceinline__ float silu(float z) { return z < -104.f ? -0.f : z * sigmoid(z); }
+__device__ __forceinline__ float silu(float z) {
+  const Logistic s(z);
+  // below -110 the rest is less than half of the smallest number
+  return z < -110.f ? -0.f : z >= 0.f ? z * s.near : z * s.e * s.near * s.scale;
+}
 __device__ __forceinline__ float silu_slope(float z) {
-  const float s = sigmoid(z);
-  return fabsf(z) > 104.f ? (z > 0.f ? 1.f : 0.f) : s * fmaf(z, 1.f - s, 1.f);
+  const Logistic s(z);
+  const float rest = s.e * s.near * s.scale;  // sigmoid(-|z|)
+  const float with = z >= 0.f ? s.near : rest, without = z >= 0.f ? rest : s.near;
+  return fabsf(z) > 110.f ? (z > 0.f ? 1.f : 0.f) : with * fmaf(z, without, 1.f);
 }
 
 // the epilogue of one column of the result
