@@ -46,9 +46,10 @@ struct Logistic {
     near = reciprocal(1.f + e * scale);
   }
 };
-// The part of the normal distribution beyond |z| on both sides, erfc(x) with x = |z| / sqrt(2), and exp(-x^2).  With
+// The part of the normal distribution beyond a = |z| on both sides, erfc(x) with x = a / sqrt(2), and exp(-a^2 / 2).  With
 // t = 3 / (3 + x), erfc(x) exp(x^2) / t is a polynomial of degree 9 in t to 8e-9 of its value, fitted to erfcx over x up
-// to 14.2; x^2 is taken in two floats, so the tail keeps its digits.
+// to 14.2; a^2 is taken in two floats, so the tail keeps its digits (from x, a rounded product, exp(-x^2) would lose 214
+// roundings at 13).
 __device__ __forceinline__ float two_tails(float a, float &gauss) {
   const float x = a * 0.70710678118654752f, t = 3.f * reciprocal(3.f + x);
   float p = 0.0516761677250975f;
@@ -61,8 +62,8 @@ __device__ __forceinline__ float two_tails(float a, float &gauss) {
   p = fmaf(p, t, 0.17356429719995523f);
   p = fmaf(p, t, 0.18843063685731984f);
   p = fmaf(p, t, 0.18804880854297287f);
-  const float q = x * x, h = -q * kLog2e;
-  gauss = exp2_sum(h, (fmaf(-q, kLog2e, -h) - q * kLog2eRest) - fmaf(x, x, -q) * kLog2e);
+  const float q = 0.5f * a * a, h = -q * kLog2e;
+  gauss = exp2_sum(h, (fmaf(-q, kLog2e, -h) - q * kLog2eRest) - fmaf(0.5f * a, a, -q) * kLog2e);
   return t * p * gauss;
 }
 // z times the normal distribution's mass below z: 0 for minus infinity

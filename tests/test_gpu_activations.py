@@ -88,3 +88,29 @@ def test_activations_of_what_is_not_finite(cl):
         assert s[0] == 1 and s[1] == 0 and np.isnan(s[2]) and s[3] == 0.5 and np.isfinite(s[4]), (act, s)
     s = _slope(cl, "relu", z)
     assert s[0] == 1 and s[1] == 0 and s[3] == 0 and s[4] == 1
+
+
+def _tails(z):
+    """the normal distribution's mass beyond |z| on one side"""
+    return 0.5 * _erfc(np.abs(z) / math.sqrt(2))
+
+
+# The tail is t p(t) exp(-z^2 / 2) / 2 with t = 3 / (3 + |z| / sqrt 2).  t is off by 5 u (a product, a sum, a reciprocal,
+# a product), which its polynomial passes on up to 3.4 times; the polynomial's own roundings come to 4 u, the
+# exponential's to 4 u, the products' to 3 u: 28 u of the tail.
+TAIL = 28 * U
+
+
+def test_gelu_of_far_values(cl):
+    z64 = Z.astype(np.float64)
+    tail = np.abs(z64) * _tails(z64)
+    want = np.maximum(z64, 0) - tail
+    _within(_forward(cl, "gelu", Z), want, TAIL * tail + 2 * U * np.abs(want) + LEAST, Z, "gelu")
+
+
+def test_slope_of_gelu_of_far_values(cl):
+    """the density is off by the exponential's 4 u and two products"""
+    z64 = Z.astype(np.float64)
+    tail, density = _tails(z64), np.abs(z64) * np.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
+    want = np.where(z64 > 0, 1 - tail + density, tail - density)
+    _within(_slope(cl, "gelu", Z), want, TAIL * tail + 7 * U * density + 2 * U * np.abs(want) + 20 * LEAST, Z, "slope of gelu")
