@@ -10,6 +10,10 @@
 // the registers of the threads that share it, 16 to 1024 of them by its width; blocks walk over rows and keep weight,
 // bias and, backward, their columns' parts of gw and gb in registers too.  The parts meet in a second launch, in block
 // order.  Wider rows than 1024 threads hold go through memory once per sum.
+//
+// The forward pass keeps the mean in two floats, of which the backward pass is given the first.  Where that lies further
+// than a standard deviation from 0, the second one moves h by more than a rounding of 1 and is summed anew (2^-24 of a
+// mean of 4096 would put all h of a row with a variance of 1 up to 2.4e-4 off).
 #include <hip/hip_runtime.h>
 
 #include <cstring>
@@ -42,6 +46,14 @@ __device__ __forceinline__ void row_sums(double &a, double &b) {
 #pragma unroll
     for (int i = 1; i < WAVES; i++) a += part[0][first + i], b += part[1][first + i];
   }
+}
+
+// Whether what the mean's rounding to fp32 lost shows in h; and that, from the sum of a row's x - mean.  A mean that is not
+// the row's own, rounded, is taken as it is.
+__device__ __forceinline__ bool far_mean(float mean, float rstd) { return fabsf(mean * rstd) > 1.f; }
+__device__ __forceinline__ float low_of_mean(double sum, double per, float mean) {
+  const float low = (float)(sum * per);
+  return fabsf(low) <= 0x1p-23f * fabsf(mean) ? low : 0.f;
 }
 
 // The elements a thread holds of a row: J units of V neighbouring ones, SPAN units apart.  V 4: a width that is a
@@ -154,7 +166,7 @@ __device__ __forceinline__ void norm_columns(const NormGradParams &P, long block
     for (long r = run; r < P.rows; r += RUNS) {
       const float gy = P.gy[r * P.gy_pitch + col];
       sb += (double)gy;
-      sw += (double)(gy * ((P.x[r * P.x_pitch + col] - P.mean[r]) * P.rstd[r]));
+      sw += (double)(gy * (((P.x[r * P.x_pitch + col] - P.mean[r]) - P.low[r]) * P.rstd[r]));
     }
   part[0][run][lane] = sw;
   part[1][run][lane] = sb;
@@ -173,13 +185,41 @@ __device__ __forceinline__ void norm_columns(const NormGradParams &P, long block
 // many parts of gw and gb as blocks of 256, two to a compute unit (2000 x 4096: 29.0 us against 33.2, 2047 x 1537: 17.8
 // against 18.8); rows past the caches by the latter, which are not held up by one another's sums (16384 x 4096: 143 us
 // against 160).
-template <int SPAN, int V, int J, bool STREAM, bool FEW>
-using HeldGrad = Held<SPAN, V, J, STREAM, FEW || STREAM ? 256 : 512>;
-// FEW rows: the first row_blocks blocks walk over the rows, the others sum columns, from the caches; nothing is folded.
-template <int SPAN, int V, int J, bool STREAM, bool FEW>
-__global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, FEW>::LANES)) void norm_grad(NormGradParams P, int row_blocks) {
-  typedef HeldGrad<SPAN, V, J, STREAM, FEW> H;
-  if constexpr (FEW) {
+enum GradKind : int { PARTS, FEW, ONLY_X };
+template <int SPAN, int V, int J, bool STREAM, GradKind KIND>
+using HeldGrad = Held<SPAN, V, J, STREAM, KIND != PARTS || STREAM ? 256 : 512>;
+// The second float of the mean of the row whose x a thread holds, 0 where it does not show.  The threads that meet at a
+// barrier decide together: all rows of the block where a row is shared by several waves.
+template <int SPAN, int V, class H>
+__device__ __forceinline__ float low_part(const NormGradParams &P, const float (&x)[H::N], float mean, float rstd, long row0, double per) {
+  const bool mine = far_mean(mean, rstd);
+  bool any = false;
+  if constexpr (H::ROWS == 1) {
+    any = mine;
+  } else if constexpr (SPAN > kWave) {
+#pragma unroll
+    for (int i = 0; i < H::ROWS; i++) {
+      const long r = row0 + i < P.rows ? row0 + i : P.rows - 1;
+      any |= far_mean(P.mean[r], P.rstd[r]);
+    }
+  } else {
+    any = __any(mine);
+  }
+  if (!any) return 0.f;
+  double sum = 0.0, none = 0.0;
+#pragma unroll
+  for (int k = 0; k < H::N; k++)
+    if (H::at(k / V) < (int)P.width) sum += (double)(x[k] - mean);
+  row_sums<SPAN, H::LANES>(sum, none);
+  return mine ? low_of_mean(sum, per, mean) : 0.f;
+}
+
+// PARTS: each block leaves its parts of gw and gb.  FEW rows: the first row_blocks blocks walk over the rows, the others
+// sum columns, from the caches; nothing is folded.  ONLY_X: rows alone.
+template <int SPAN, int V, int J, bool STREAM, GradKind KIND>
+__global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, KIND>::LANES)) void norm_grad(NormGradParams P, int row_blocks) {
+  typedef HeldGrad<SPAN, V, J, STREAM, KIND> H;
+  if constexpr (KIND == FEW) {
     if ((int)blockIdx.x >= row_blocks) {
       norm_columns<H::LANES>(P, blockIdx.x - row_blocks);
       return;
@@ -187,38 +227,47 @@ __global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, FEW>::LANES)) void no
   }
   const int width = (int)P.width;
   const double per = 1.0 / (double)width;
-  // a block of 1024 threads is alone on its compute unit and requests the next row before it works on this one
+  // a block of 1024 threads is alone on its compute unit and requests the next row, and its statistics, before it works on
+  // this one (8192 x 8192: 152 us, 164 without the statistics)
   constexpr bool AHEAD = SPAN == 1024;
   float w[H::N];
   double gw[H::N], gb[H::N];
   H::load_steps(w, P.w, P.w_step, width, 1.f);
 #pragma unroll
   for (int k = 0; k < H::N; k++) gw[k] = gb[k] = 0.0;
-  float h[H::N], gy[H::N], next_h[AHEAD ? H::N : 1], next_gy[AHEAD ? H::N : 1];
+  float h[H::N], gy[H::N], next_h[AHEAD ? H::N : 1], next_gy[AHEAD ? H::N : 1], next_mean = 0.f, next_rstd = 0.f;
   auto request = [&](float (&a)[H::N], float (&b)[H::N], long r) {
     r = r < P.rows ? r : P.rows - 1;
     H::load(a, P.x + r * P.x_pitch, width);
     H::load(b, P.gy + r * P.gy_pitch, width);
   };
-  if constexpr (AHEAD) request(next_h, next_gy, blockIdx.x);
+  auto statistics = [&](float &mean, float &rstd, long r) {
+    r = r < P.rows ? r : P.rows - 1;
+    mean = P.mean[r], rstd = P.rstd[r];
+  };
+  if constexpr (AHEAD) request(next_h, next_gy, blockIdx.x), statistics(next_mean, next_rstd, blockIdx.x);
   for (long row0 = (long)blockIdx.x * H::ROWS; row0 < P.rows; row0 += (long)row_blocks * H::ROWS) {
-    const long row = row0 + threadIdx.x / SPAN;
+    const long row = row0 + (H::ROWS > 1 ? threadIdx.x / SPAN : 0);
     const bool real = row < P.rows;
-    const long from = real ? row : P.rows - 1;
+    float mean, rstd, low;
     if constexpr (AHEAD) {
+      mean = next_mean, rstd = next_rstd;
 #pragma unroll
       for (int k = 0; k < H::N; k++) h[k] = next_h[k], gy[k] = next_gy[k];
       request(next_h, next_gy, row + row_blocks);
+      statistics(next_mean, next_rstd, row + row_blocks);
     } else {
       request(h, gy, row);
+      statistics(mean, rstd, row);
     }
-    const float mean = P.mean[from], rstd = P.rstd[from];
+    if constexpr (KIND == FEW) low = P.low[real ? row : P.rows - 1];
+    else low = low_part<SPAN, V, H>(P, h, mean, rstd, row0, per);
     double s1 = 0.0, s2 = 0.0;
 #pragma unroll
     for (int k = 0; k < H::N; k++) {
-      h[k] = (h[k] - mean) * rstd;
+      h[k] = ((h[k] - mean) - low) * rstd;
       const float part = gy[k] * h[k], g = gy[k] * w[k];
-      if (!FEW && real) gw[k] += (double)part, gb[k] += (double)gy[k];
+      if (KIND == PARTS && real) gw[k] += (double)part, gb[k] += (double)gy[k];
       gy[k] = g;
       if (H::at(k / V) < width) s1 += (double)g, s2 += (double)(g * h[k]);
     }
@@ -229,7 +278,7 @@ __global__ __launch_bounds__((HeldGrad<SPAN, V, J, STREAM, FEW>::LANES)) void no
     for (int k = 0; k < H::N; k++) h[k] = (gy[k] - c1 - h[k] * c2) * rstd;
     if (real) H::store(h, P.gx + row * P.gx_pitch, width);
   }
-  if (FEW || !P.parts) return;
+  if (KIND != PARTS || !P.parts) return;
   if constexpr (H::ROWS > 1) {  // the waves' parts, in wave order
     __shared__ double sums[2][SPAN * V * J];
     for (int s = 0; s < H::ROWS; s++) {
@@ -316,13 +365,13 @@ __global__ __launch_bounds__(kWide) void norm_wide(NormParams P) {
 __device__ __forceinline__ void norm_grad_wide_row(const NormGradParams &P, long row) {
   const float *x = P.x + row * P.x_pitch, *gy = P.gy + row * P.gy_pitch;
   float *gx = P.gx + row * P.gx_pitch;
-  const float mean = P.mean[row], rstd = P.rstd[row];
+  const float mean = P.mean[row], rstd = P.rstd[row], low = P.low[row];
   double s1 = 0.0, s2 = 0.0;
 #pragma unroll 4
   for (long i = threadIdx.x; i < P.width; i += kWide) {
     const float g = gy[i] * (P.w ? P.w[i * P.w_step] : 1.f);
     s1 += (double)g;
-    s2 += (double)(g * ((x[i] - mean) * rstd));
+    s2 += (double)(g * (((x[i] - mean) - low) * rstd));
   }
   row_sums<kWide, kWide>(s1, s2);
   const double per = 1.0 / (double)P.width;
@@ -330,7 +379,26 @@ __device__ __forceinline__ void norm_grad_wide_row(const NormGradParams &P, long
 #pragma unroll 4
   for (long i = threadIdx.x; i < P.width; i += kWide) {
     const float g = gy[i] * (P.w ? P.w[i * P.w_step] : 1.f);
-    gx[i] = (g - c1 - ((x[i] - mean) * rstd) * c2) * rstd;
+    gx[i] = (g - c1 - (((x[i] - mean) - low) * rstd) * c2) * rstd;
+  }
+}
+
+// The second floats of the rows' means, for those who look at a row's elements one by one: a block to a row, which is read
+// where they show.
+constexpr int kLow = 256;
+__global__ __launch_bounds__(kLow) void norm_low(NormGradParams P) {
+  for (long row = blockIdx.x; row < P.rows; row += gridDim.x) {
+    const float mean = P.mean[row];
+    float low = 0.f;
+    if (far_mean(mean, P.rstd[row])) {
+      const float *x = P.x + row * P.x_pitch;
+      double sum = 0.0, none = 0.0;
+#pragma unroll 4
+      for (long i = threadIdx.x; i < P.width; i += kLow) sum += (double)(x[i] - mean);
+      row_sums<kLow, kLow>(sum, none);
+      low = low_of_mean(sum, 1.0 / (double)P.width, mean);
+    }
+    if (threadIdx.x == 0) P.low[row] = low;
   }
 }
 
@@ -413,25 +481,36 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
   NormGradParams P = given;
   const bool past = 12 * P.rows * P.width > kStreamBytes, columns = P.gw || P.gb;
   // Up to 1024 rows a second look at them from the caches is cheaper than the blocks' parts of gw and gb, which are then
-  // as large as the rows, and a second launch (500 x 4096: 10.6 us against 26.7, 1000 x 4096: 19.4 against 27.5,
-  // 2000 x 4096: 41 against 29).  Without gw and gb there is nothing to leave.
+  // as large as the rows (500 x 4096: 12.6 us against 26.7, 1000 x 4096: 20.8 against 27.5, 2000 x 4096: 43 against 29).
+  // Without gw and gb there is nothing to leave.  2.5 us of it are the launch that looks for far means.
   const bool few = P.rows <= 1024 || (!columns && !past);
   long blocks = 0;
+  auto find_low = [&] {
+    P.low = (float *)thcl_rt_workspace(rt, (size_t)P.rows * sizeof(float));
+    THCL_CHECK(P.low != nullptr, "layerNormBackward workspace: %s", thcl_rt_error());
+    hipLaunchKernelGGL(norm_low, dim3(blocks_of(P.rows)), dim3(kLow), 0, stream, P);
+    check_launch("layerNormBackward");
+  };
   auto with = [&](auto v) {
     return [&](auto span, auto j) {
       constexpr int SPAN = decltype(span)::value, V = decltype(v)::value, J = decltype(j)::value;
       if (few) {
-        typedef HeldGrad<SPAN, V, J, false, true> H;
+        typedef HeldGrad<SPAN, V, J, false, FEW> H;
         const long want = (P.rows + H::ROWS - 1) / H::ROWS;
-        const long rows = P.gx ? want : 0, cols = columns ? (P.width + (H::LANES == 256 ? 16 : 32) - 1) / (H::LANES == 256 ? 16 : 32) : 0;
+        if (!columns) {
+          if (P.gx) hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, ONLY_X>), dim3((unsigned)want), dim3(H::LANES), 0, stream, P, (int)want);
+          return;
+        }
+        find_low();
+        const long rows = P.gx ? want : 0, cols = (P.width + (H::LANES == 256 ? 16 : 32) - 1) / (H::LANES == 256 ? 16 : 32);
         auto launch = [&](long r, long c) {
-          if (r + c > 0) hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, true>), dim3((unsigned)(r + c)), dim3(H::LANES), 0, stream, P, (int)r);
+          if (r + c > 0) hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, FEW>), dim3((unsigned)(r + c)), dim3(H::LANES), 0, stream, P, (int)r);
         };
         if (P.gx == P.gy || P.gx == P.x) launch(0, cols), launch(rows, 0);  // the columns' operands are about to be overwritten
         else launch(rows, cols);
         return;
       }
-      const int lanes = past ? HeldGrad<SPAN, V, J, true, false>::LANES : HeldGrad<SPAN, V, J, false, false>::LANES;
+      const int lanes = past ? HeldGrad<SPAN, V, J, true, PARTS>::LANES : HeldGrad<SPAN, V, J, false, PARTS>::LANES;
       const long want = (P.rows + lanes / SPAN - 1) / (lanes / SPAN), most = (long)cus * (lanes > 256 ? 1 : 2);
       blocks = want < most ? want : most;
       if (columns) {
@@ -439,8 +518,8 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
         THCL_CHECK(P.parts != nullptr, "layerNormBackward workspace: %s", thcl_rt_error());
       }
       const dim3 grid((unsigned)blocks), block(lanes);
-      if (past) hipLaunchKernelGGL((norm_grad<SPAN, V, J, true, false>), grid, block, 0, stream, P, (int)blocks);
-      else hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, false>), grid, block, 0, stream, P, (int)blocks);
+      if (past) hipLaunchKernelGGL((norm_grad<SPAN, V, J, true, PARTS>), grid, block, 0, stream, P, (int)blocks);
+      else hipLaunchKernelGGL((norm_grad<SPAN, V, J, false, PARTS>), grid, block, 0, stream, P, (int)blocks);
     };
   };
   bool fits;
@@ -452,6 +531,7 @@ void thcl_norm_backward(THClState *state, thcl_rt *rt, const NormGradParams &giv
     check_launch("layerNormBackward");
     if (P.parts) hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * P.width + kFoldCols - 1) / kFoldCols)), dim3(kFoldRuns * kFoldCols), 0, stream, P, (int)blocks);
   } else {
+    find_low();
     if (columns)  // first: gx may take the place of gy or x
       hipLaunchKernelGGL(norm_grad_columns, dim3(blocks_of((P.width + 31) / 32)), dim3(kWide), 0, stream, P);
     check_launch("layerNormBackward");

@@ -15,7 +15,9 @@ struct NormGradParams {
   const float *gy, *x, *mean, *rstd, *w;
   float *gx, *gw, *gb;
   long rows, width, gy_pitch, x_pitch, gx_pitch, w_step, gw_step, gb_step;
-  double *parts;  // set by thcl_norm_backward: [block][gw, gb][width]
+  // set by thcl_norm_backward: [block][gw, gb][width], and the second floats of the means
+  double *parts;
+  float *low;
 };
 
 void thcl_norm(THClState *state, thcl_rt *rt, const NormParams &P);

@@ -554,7 +554,8 @@ void THClBlas_ger(THClState *state, long m, long n, float alpha, THClTensor *x, 
  * statistics for the backward pass, or are NULL.  self may be src. */
 void THClTensor_layerNorm(THClState *state, THClTensor *self, THClTensor *mean, THClTensor *rstd, THClTensor *src,
                           THClTensor *weight, THClTensor *bias, float eps);
-/* Gradients by the input, the weight and the bias, each or NULL.  gradInput may be gradOutput or src. */
+/* Gradients by the input, the weight and the bias, each or NULL.  gradInput may be gradOutput or src.  mean and rstd are
+ * what the forward pass kept; what a mean far from 0 lost when it was rounded is found again in src. */
 void THClTensor_layerNormBackward(THClState *state, THClTensor *gradInput, THClTensor *gradWeight, THClTensor *gradBias,
                                   THClTensor *gradOutput, THClTensor *src, THClTensor *mean, THClTensor *rstd,
                                   THClTensor *weight);
