@@ -74,6 +74,7 @@ void THClTensor_layerNorm(THClState *state, THClTensor *self, THClTensor *mean, 
   thcl_check_apart(self, whole, src, true, "the result");
   THClTensor *results[3] = {self, mean, rstd}, *operands[3] = {src, weight, bias};
   for (int r = 0; r < 3; r++) {
+    thcl_check_distinct(results[r], r == 0 ? whole : per_row);
     for (int o = r == 0 ? 1 : 0; o < 3; o++) thcl_check_apart(results[r], r == 0 ? whole : per_row, operands[o], false, "a result");
     for (int q = 0; q < r; q++) thcl_check_apart(results[r], per_row, results[q], false, "a result");
   }
@@ -133,6 +134,7 @@ void THClTensor_layerNormBackward(THClState *state, THClTensor *gradInput, THClT
   feature.size[0] = width;
   THClTensor *results[3] = {gradInput, gradWeight, gradBias}, *operands[5] = {gradOutput, src, mean, rstd, weight};
   for (int r = 0; r < 3; r++) {
+    thcl_check_distinct(results[r], r == 0 ? whole : feature);
     // an element of the input's gradient goes where the same element of gradOutput or of the input may have been
     for (int o = 0; o < 5; o++) thcl_check_apart(results[r], r == 0 ? whole : feature, operands[o], r == 0 && o < 2, "a result");
     for (int q = 0; q < r; q++) thcl_check_apart(results[r], feature, results[q], false, "a result");
@@ -187,6 +189,7 @@ void THClTensor_linear(THClState *state, THClTensor *self, THClTensor *preact, T
   check_int(K);
   THClTensor *results[2] = {self, preact}, *operands[4] = {src, weight, bias, residual};
   for (int r = 0; r < 2; r++) {
+    thcl_check_distinct(results[r], shape);
     // the sum may take the residual's place: each of its elements is read by the lane that writes there
     for (int o = 0; o < 4; o++) thcl_check_apart(results[r], shape, operands[o], r == 0 && o == 3, "a result");
     if (r == 1) thcl_check_apart(preact, shape, self, false, "a result");
@@ -255,6 +258,7 @@ void THClTensor_linearBackward(THClState *state, THClTensor *gradInput, THClTens
   THClTensor *results[3] = {gradInput, gradWeight, gradBias}, *operands[4] = {gradOutput, src, weight, slope ? preact : nullptr};
   const Shape *shapes[3] = {&in, &w_shape, &b_shape};
   for (int r = 0; r < 3; r++) {
+    thcl_check_distinct(results[r], *shapes[r]);
     for (int o = 0; o < 4; o++) thcl_check_apart(results[r], *shapes[r], operands[o], false, "a result");
     for (int q = 0; q < r; q++) thcl_check_apart(results[r], *shapes[r], results[q], false, "a result");
   }
@@ -332,12 +336,12 @@ void THClTensor_groupedmm(THClState *state, THClTensor *self, THClTensor *src, T
   check_int(K);
   Shape shape = shape2(T, N);
   THClTensor *operands[3] = {src, weight, sizes};
+  thcl_check_distinct(self, shape);
   for (int o = 0; o < 3; o++) thcl_check_apart(self, shape, operands[o], false, "the result");
   shape.give(state, self);
   RowsIn x(state, src);
   MatrixIn w(state, weight);
   ThclTemp s(state, THClTensor_newContiguous(state, sizes));
-  THCL_CHECK(!thcl_overlapping(self), "the result must not repeat its elements");
   // rows that belong to no group keep what they hold, so a stand-in begins as a copy
   Rows y;
   ThclTemp dense(state, nullptr);
@@ -383,6 +387,8 @@ void THClTensor_groupedmmBackward(THClState *state, THClTensor *gradInput, THClT
     thcl_check_apart(gradWeight, w_shape, operands[o], false, "a result");
   }
   thcl_check_apart(gradWeight, w_shape, gradInput, false, "a result");
+  thcl_check_distinct(gradInput, in);
+  thcl_check_distinct(gradWeight, w_shape);
   if (gradInput) {  // the same product with each group's matrix transposed
     ThclTemp wt(state, THClTensor_newTranspose(state, weight, 1, 2));
     THClTensor_groupedmm(state, gradInput, gradOutput, wt.t, sizes);
@@ -394,7 +400,7 @@ void THClTensor_groupedmmBackward(THClState *state, THClTensor *gradInput, THClT
     ThclTemp s(state, THClTensor_newContiguous(state, sizes));
     ThclTemp dense(state, nullptr);
     THClTensor *w = gradWeight;
-    if (thcl_overlapping(w) || (w->size[2] > 1 && w->stride[2] != 1)) {
+    if (w->size[2] > 1 && w->stride[2] != 1) {
       w = dense.t = THClTensor_newClone(state, gradWeight);  // what sizes that are refused leave as it was
     }
     thcl_rt *rt = thcl_ctx(state, THClTensor_getDevice(state, src));

@@ -3,6 +3,8 @@
 // pitch are used as they are, others through a dense stand-in.
 #pragma once
 
+#include <numeric>
+
 #include "internal.h"
 
 // count rows of width elements, unit stride inside a row, pitch elements from row to row
@@ -112,13 +114,28 @@ inline void thcl_check_apart(const THClTensor *out, const Shape &shape, const TH
   thcl_throw("%s must not share memory with an operand", what);
 }
 
-// The results of one call, once they have their shapes: apart from one another, and vectors among them with an
-// element per entry (a view that repeats one element has nowhere to put them).
-inline void thcl_check_results(int n, THClTensor *const *results) {
-  for (int r = 0; r < n; r++) {
-    if (!results[r]) continue;
-    if (results[r]->nDimension == 1) THCL_CHECK(results[r]->size[0] == 1 || results[r]->stride[0] != 0, "a result must not repeat its elements");
-    for (int q = 0; q < r; q++)
-      if (results[q]) thcl_check_apart(results[r], Shape(results[r]), results[q], false, "a result");
+// Refuses, before anything is changed, a result that has its shape already and repeats elements: what it held afterwards
+// would hang on the order of writes.
+inline void thcl_check_distinct(const THClTensor *out, const Shape &shape) {
+  if (!out || !shape.same_as(out) || !thcl_overlapping(out)) return;
+  // two dimensions whose steps interleave may still meet nowhere: they do at the steps' smallest common multiple
+  long size[2], step[2];
+  int k = 0;
+  for (int d = 0; d < out->nDimension; d++) {
+    if (out->size[d] == 1) continue;
+    if (k < 2) size[k] = out->size[d], step[k] = out->stride[d];
+    k++;
   }
+  if (k == 2 && step[0] > 0 && step[1] > 0) {
+    const long g = std::gcd(step[0], step[1]);
+    if (step[1] / g >= size[0] || step[0] / g >= size[1]) return;
+  }
+  thcl_throw("a result must not repeat its elements");
+}
+
+// The results of one call, once they have their shapes: apart from one another.
+inline void thcl_check_results(int n, THClTensor *const *results) {
+  for (int r = 0; r < n; r++)
+    for (int q = 0; q < r; q++)
+      if (results[r] && results[q]) thcl_check_apart(results[r], Shape(results[r]), results[q], false, "a result");
 }

@@ -546,8 +546,9 @@ void THClBlas_ger(THClState *state, long m, long n, float alpha, THClTensor *x, 
 /* ------------------------------------------------------------------------- */
 /* Layers of a network (no counterpart in the reference, whose users compose   */
 /* them from addmm, sum and the pointwise operators).  Results are resized;    */
-/* they must not share memory with an operand unless said otherwise.  NULL     */
-/* stands for an operand or a result that is not there.                        */
+/* they must not repeat elements (expanded views), nor share memory with an    */
+/* operand unless said otherwise.  NULL stands for an operand or a result that */
+/* is not there.                                                               */
 /* ------------------------------------------------------------------------- */
 /* Layer norm over the last dimension: self = (src - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps);
  * weight and bias are vectors or NULL (1 and 0).  mean and rstd, of src's shape without its last dimension, keep the
