@@ -302,24 +302,29 @@ __device__ __forceinline__ bool find_work(const Product &P, int tile_rows, int r
   return w.row0 < w.rows;
 }
 
-// Products whose pitches are too long for the tiled kernel's 32-bit offsets.
+// Products whose pitches are too long for the tiled kernel's 32-bit offsets: tiles of 64 x 128, which the blocks walk over.
 constexpr int kDirectM = 64, kDirectN = 128;
-__global__ __launch_bounds__(256) void product_far(Product P) {
+__global__ __launch_bounds__(256) void product_far(Product P, int row_tiles) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  Work w;
-  if (!find_work(P, kDirectM, blockIdx.x, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0, w)) return;
-  const int row0 = w.row0 + (wave / 2) * 32, col0 = blockIdx.y * kDirectN + (wave % 2) * 64;
-  if (row0 >= w.rows || col0 >= P.n) return;
+  for (int tile = blockIdx.x; tile < row_tiles; tile += gridDim.x) {
+    Work w;
+    if (!find_work(P, kDirectM, tile, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0, w)) return;
+    const int row0 = w.row0 + (wave / 2) * 32;
+    if (row0 >= w.rows) continue;
+    for (int col_tile = blockIdx.y; col_tile * (long)kDirectN < P.n; col_tile += gridDim.y) {
 #pragma unroll 1
-  for (int j = 0; j < 2; j++) {
-    const f16v acc = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0, 1, col0 + 32 * j, 1, w.k0, w.k1);
-    const int col = col0 + 32 * j + lane % 32;
-    if (col >= P.n) continue;
-    const Column line(P, col);
+      for (int j = 0; j < 2; j++) {
+        const int col0 = col_tile * kDirectN + (wave % 2) * 64 + 32 * j, col = col0 + lane % 32;
+        if (col0 >= P.n) continue;
+        const f16v acc = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0, 1, col0, 1, w.k0, w.k1);
+        if (col >= P.n) continue;
+        const Column line(P, col);
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-      const int row = row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-      if (row < w.rows) line.finish(P, w.c, row, acc[r]);
+        for (int r = 0; r < 16; r++) {
+          const int row = row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+          if (row < w.rows) line.finish(P, w.c, row, acc[r]);
+        }
+      }
     }
   }
 }
@@ -1136,6 +1141,7 @@ constexpr TileCost kTiles[4] = {{256, 256, 1, 1.51, 2.07, 7.8}, {128, 128, 2, 0.
 // the ragged products, fitted to 12 shapes with groups of random sizes, 2 % over the best choice
 constexpr TileCost kRowTiles[4] = {{256, 256, 1, 1.48, 2.14, 7.8}, {128, 128, 2, 0.81, 1.43, 4.8}, {64, 128, 3, 0.55, 1.21, 3.6}, {32, 128, 4, 0.45, 1.31, 2.0}};
 constexpr TileCost kDepthTiles[4] = {{256, 256, 1, 1.20, 2.80, 6.7}, {128, 128, 2, 1.26, 1.91, 4.4}, {64, 128, 3, 0.84, 1.54, 4.4}, {32, 128, 4, 0.73, 1.55, 2.7}};
+constexpr int kTileThreads[4] = {Tile256::TH, Tile128::TH, Tile64::TH, Tile32::TH};
 struct ThinCost {
   double alone, chip;  // bytes per nanosecond
 };
@@ -1164,6 +1170,7 @@ ThclProductPlan thcl_product_plan(const Product &P, bool few_rows_fit, int cus) 
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {  // blocks to a tile
       if (s > 1 && slabs / s < 4) break;
       if (P.ragged == WHOLE) {
+        if (tiles * kTileThreads[t] > UINT32_MAX) break;  // a launch's threads are counted in 32 bits
         if (s > 1 && s * outputs * 4 > 1e9) break;
         const double per = tiles * s * share / 256., whole = per > 1 ? std::ceil(per) : per;
         const double turns = std::floor(whole / c.resident), rest = whole - turns * c.resident;
@@ -1252,6 +1259,7 @@ static void launch_split(const Product &P, bool akc, bool bkc, int blocks, hipSt
   const long tiles_m = (P.m - 1) / T::BM + 1, tiles_n = (P.n - 1) / T::BN + 1;
   THCL_CHECK(tiles_m * tiles_n <= INT32_MAX, THCL_DIM_WARNING);
   if (P.ragged == WHOLE) {
+    THCL_CHECK(tiles_m * tiles_n * T::TH <= UINT32_MAX, THCL_DIM_WARNING);
     const dim3 grid((unsigned)(tiles_m * tiles_n), 1, P.slices);
     if (akc && bkc) hipLaunchKernelGGL((product_split<T, true, true, false>), grid, block, 0, stream, P);
     else if (akc) hipLaunchKernelGGL((product_split<T, true, false, false>), grid, block, 0, stream, P);
@@ -1288,9 +1296,9 @@ void thcl_product(THClState *state, thcl_rt *rt, const Product &given, const cha
   const bool akc = P.a_k == 1 || P.k == 1, amc = P.a_m == 1 || P.m == 1, bkc = P.b_k == 1 || P.k == 1, bnc = P.b_n == 1 || P.n == 1;
   const long a_pitch = akc ? P.a_m : P.a_k, b_pitch = bkc ? P.b_n : P.b_k;
   if (a_pitch >= kFarPitch || b_pitch >= kFarPitch || !(akc ? bkc || bnc : amc && bnc)) {
-    const unsigned gy = (unsigned)((P.n + kDirectN - 1) / kDirectN);
-    THCL_CHECK(gy <= 65535, THCL_DIM_WARNING);
-    hipLaunchKernelGGL(product_far, dim3((unsigned)row_tiles(kDirectM), gy, P.ragged == DEPTH ? P.groups : 1), dim3(256), 0, stream, P);
+    const long down = row_tiles(kDirectM), across = (P.n - 1) / kDirectN + 1;
+    const dim3 grid((unsigned)(down < kMostBlocks ? down : kMostBlocks), (unsigned)(across < 65535 ? across : 65535), P.ragged == DEPTH ? P.groups : 1);
+    hipLaunchKernelGGL(product_far, grid, dim3(256), 0, stream, P, (int)down);
     check_launch(what);
     thcl_after_launch(state, rt);
     return;
