@@ -1058,7 +1058,8 @@ class ClTensor:
     def groupedmm(self, src: "ClTensor", weight: "ClTensor", sizes) -> "ClTensor":
         """``res:groupedmm(src, weight, sizes)``: rows of src lie group after group, ``sizes[g]`` of them each, and are
         multiplied by their group's matrix of weight ``[groups, in, out]``.  Rows of res behind the last group are left
-        as they were.  Sizes (a ClTensor, or a list of numbers) that do not fit the rows are reported by the next wait."""
+        as they were.  Sizes (a ClTensor, or a list of numbers, held as fp32) that do not fit the rows are reported by the
+        next wait."""
         sizes = _sizes_of(sizes)
         _call("THClTensor_groupedmm", self._h, src._h, weight._h, sizes._h)
         return self
@@ -1167,7 +1168,14 @@ def _handle_of(t: Optional[ClTensor]):
 
 
 def _sizes_of(sizes) -> ClTensor:
-    return sizes if isinstance(sizes, ClTensor) else ClTensor(np.asarray(sizes, dtype=np.float32).reshape(-1))
+    if isinstance(sizes, ClTensor):
+        return sizes
+    given = np.asarray(sizes, dtype=np.float64).reshape(-1)
+    with np.errstate(over="ignore"):
+        held = given.astype(np.float32)
+    if (np.abs(given[held != given]) > 2 ** 24).any():
+        raise ClError("group sizes beyond 2^24 must be numbers that fp32 holds")
+    return ClTensor(held)
 
 
 def layerNormBackward(gradInput: Optional[ClTensor], gradWeight: Optional[ClTensor], gradBias: Optional[ClTensor], gradOutput: ClTensor,
