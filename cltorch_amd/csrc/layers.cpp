@@ -69,6 +69,7 @@ void THClTensor_layerNorm(THClState *state, THClTensor *self, THClTensor *mean, 
   const long width = src->size[src->nDimension - 1];
   check_features(weight, width, 6, "vector with an entry per feature expected");
   check_features(bias, width, 7, "vector with an entry per feature expected");
+  THCL_CHECK(leading(src) <= INT32_MAX, THCL_DIM_WARNING);
   const Shape whole(src);
   Shape per_row = row_shape(src);
   thcl_check_apart(self, whole, src, true, "the result");
@@ -107,7 +108,6 @@ void THClTensor_layerNorm(THClState *state, THClTensor *self, THClTensor *mean, 
   P.x_pitch = x.pitch;
   P.y_pitch = y.pitch;
   P.eps = eps;
-  THCL_CHECK(P.rows <= INT32_MAX, THCL_DIM_WARNING);
   thcl_rt *rt = thcl_ctx(state, THClTensor_getDevice(state, src));
   thcl_norm(state, rt, P);
   y.finish();
