@@ -1388,13 +1388,15 @@ void thcl_slope(THClState *state, thcl_rt *rt, const SlopeParams &given) {
     THCL_CHECK(P.parts != nullptr, "linearBackward workspace: %s", thcl_rt_error());
   }
   const dim3 grid((unsigned)across, (unsigned)parts), block(256);
+  // without an activation gz is gy itself
+  if (P.act == THCL_ACT_NONE) hipLaunchKernelGGL((slope_columns<THCL_ACT_NONE, false, true>), grid, block, 0, stream, P);
 #define GO(ACT)                                                                                                  \
   if (P.act == ACT) {                                                                                            \
     if (P.gz && P.gb) hipLaunchKernelGGL((slope_columns<ACT, true, true>), grid, block, 0, stream, P);           \
     else if (P.gz) hipLaunchKernelGGL((slope_columns<ACT, true, false>), grid, block, 0, stream, P);             \
     else hipLaunchKernelGGL((slope_columns<ACT, false, true>), grid, block, 0, stream, P);                       \
   }
-  GO(THCL_ACT_NONE) GO(THCL_ACT_RELU) GO(THCL_ACT_GELU) GO(THCL_ACT_SILU)
+  GO(THCL_ACT_RELU) GO(THCL_ACT_GELU) GO(THCL_ACT_SILU)
 #undef GO
   check_launch("linearBackward");
   if (P.gb) {
