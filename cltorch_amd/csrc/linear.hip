@@ -340,6 +340,8 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 
+constexpr unsigned kTiny = (17u << 24) - 1u;  // Feed::least of 2^-110
+
 constexpr int KS = 16;      // k per slab: two chunks of 8, one matrix instruction deep
 constexpr int CHUNKS = KS / 8;
 
@@ -380,6 +382,24 @@ struct Feed {
   int row_bytes;          // along k, when the lines are contiguous
   int to[N];              // where the piece goes in LDS
   unsigned least = ~0u;   // smallest magnitude met: its bits shifted up by one, less one (zero counts as the largest)
+  // the line of a thread's only piece
+  static __device__ __forceinline__ int line() {
+    static_assert(N == 1, "a thread stays with one line");
+    const int f = threadIdx.x % PIECES;
+    return KC ? f / PER_LINE : f % LINES;
+  }
+  // the largest magnitude that this thread loads for `steps` slabs, from begin() on; NaN counts for nothing
+  __device__ __forceinline__ float largest(int steps) {
+    float most = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < steps; s++) {
+      float x[N][E];
+      load(x);
+#pragma unroll
+      for (int e = 0; e < E; e++) most = fmaxf(most, fabsf(x[0][e]));
+    }
+    return most;
+  }
   static __device__ __forceinline__ int piece(int i) {
     const int f = (threadIdx.x + TH * i) % PIECES;  // threads beyond the last piece repeat one: no branch around loads
     return KC ? f % PER_LINE : f / LINES;
@@ -681,25 +701,63 @@ __device__ __forceinline__ void split_block(const Product &P, int block, int blo
       }
     }
 
-    // What does not split is taken again with fp32 products.  A value that is not finite (or rounds to an infinity) leaves
-    // NaN among its parts, which shows in every result it belongs to; the others stay as they are.  A value below 2^-110
-    // has bits below bf16's smallest, 2^-133; the staging threads have looked out for those.
-    const bool tiny = __syncthreads_or(min(fa.least, fb.least) < (17u << 24) - 1u);  // and LDS is taken for the results below
+    // What does not split is taken again with fp32 products, in tiles of 32 x 32.  A value that is not finite (or rounds to
+    // an infinity) leaves NaN among its parts, which shows in every result it belongs to; the others stay as they are.  A
+    // value below 2^-110 has bits below bf16's smallest, 2^-133, and its parts are off by up to 2^-134 of 1.  Over all k
+    // that comes to less than 2^-133 depth largest in the results of its line, largest being of both operands' values: a
+    // result 2^25 times that keeps all of its digits, smaller ones are taken again.  The staging threads have looked out for
+    // such values, each for its line; only then the operands are gone through once more for the largest.  (2048 x 4096 x
+    // 4096 with such a value in every row: 412 us, with a whole row of them 854, without any 345; with all of the tiles
+    // taken again 3860.)
+    const bool tiny = __syncthreads_or(min(fa.least, fb.least) < kTiny);  // and LDS is taken for the results below
     const bool inside = row0 < w.rows && wcol0 < P.n;  // the same for a wave
     const int colb = wcol0 + NT * (lane % 32);
+    auto row_of = [&](int i, int r) { return row0 + MT * (8 * (r / 4) + 4 * (lane / 32) + r % 4) + i; };
+    unsigned low_rows[MT] = {}, low_cols = 0;  // bits r and j: results of lines with such values
+    float bound = 0.f;
+    if (tiny) {
+      int *flags = (int *)lds0;
+      float *most = (float *)lds1;
+      for (int i = threadIdx.x; i < T::BM + T::BN; i += T::TH) flags[i] = 0;
+      __syncthreads();
+      if (fa.least < kTiny) flags[FA::line()] = 1;
+      if (fb.least < kTiny) flags[T::BM + FB::line()] = 1;
+      fa.begin(P.a, P.a_m, P.a_k, w.row0, w.rows, w.k0, w.k1);
+      fb.begin(w.b, P.b_n, P.b_k, col0, P.n, w.k0, w.k1);
+      float largest = fmaxf(fa.largest(steps), fb.largest(steps));
+#pragma unroll
+      for (int d = kWave / 2; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d, kWave));
+      if (lane == 0) most[wave] = largest;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < T::WM * T::WN; v++) largest = fmaxf(largest, most[v]);
+      bound = 0x1p-108f * (float)depth * largest;
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) low_rows[i] |= (unsigned)flags[row_of(i, r) - w.row0] << r;
+#pragma unroll
+      for (int j = 0; j < NT; j++) low_cols |= (unsigned)flags[T::BM + colb + j - col0] << j;
+      __syncthreads();
+    }
     if (inside) {
 #pragma unroll
       for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          bool again = tiny;
+          auto lost = [&](int r) { return ((low_rows[i] >> r | low_cols >> j) & 1) && fabsf(acc[i][j][r]) < bound; };
+          auto real = [&](int r) { return row_of(i, r) < w.rows && colb + j < P.n; };
+          bool again = false;
 #pragma unroll
-          for (int r = 0; r < 16; r++)
-            again |= row0 + MT * (8 * (r / 4) + 4 * (lane / 32) + r % 4) + i < w.rows && colb + j < P.n && !(fabsf(acc[i][j][r]) < INFINITY);
+          for (int r = 0; r < 16; r++) again |= real(r) && !(fabsf(acc[i][j][r]) < INFINITY);
+          if (tiny) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) again |= real(r) && lost(r);
+          }
           if (__any(again)) {
             const f16v v = product_direct(P.a, P.a_m, P.a_k, w.rows, w.b, P.b_n, P.b_k, P.n, row0 + i, MT, wcol0 + j, NT, w.k0, w.k1);
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[i][j][r] = tiny || !(fabsf(acc[i][j][r]) < INFINITY) ? v[r] : acc[i][j][r];
+            for (int r = 0; r < 16; r++) acc[i][j][r] = lost(r) || !(fabsf(acc[i][j][r]) < INFINITY) ? v[r] : acc[i][j][r];
           }
         }
     }
@@ -995,13 +1053,14 @@ __global__ __launch_bounds__(64 * kThinWaves, 2) void product_thin(Product P) {
   stream.run(P, w, col0, s0, s1, acc);
   gather();
   if constexpr (SPLIT) {
-    // what does not split is taken again with fp32 products, as in product_split
+    // what does not split is taken again with fp32 products, as in product_split, but all of a block's results together
+    // (64 x 4096 x 16384: 156 us with a single value below 2^-110, 80 without)
     bool again = false;
 #pragma unroll
     for (int t = 0; t < MT; t++)
 #pragma unroll
       for (int h = 0; h < 2; h++) again |= w.row0 + 16 * t + wave + 8 * h < w.rows && col < P.n && !(fabsf(sums[t][h]) < INFINITY);
-    const bool tiny = __syncthreads_or(stream.least < (17u << 24) - 1u);
+    const bool tiny = __syncthreads_or(stream.least < kTiny);
     if (__syncthreads_or(again || tiny)) {
       float old[MT][2];
 #pragma unroll
