@@ -470,8 +470,9 @@ struct Feed {
 
 // BM x BN results by WM x WN waves, START: slabs that its first loads and its epilogue are worth.  Two waves or more to
 // a SIMD, so that one's matrix instructions run under the vector instructions with which another splits its operands:
-// 128 x 128 by eight waves with 4 values of k each takes 50 us for 1531 x 1027 x 2053, by four with 8 it took 61; 64 x
-// 128 by eight waves loses, 59 us against 55 at 1536 x 1024 x 2048.
+// 128 x 128 by eight waves with 4 values of k each takes 51 us for 1531 x 1027 x 2053, by four with 8 it took 61 (the
+// product alone; with gelu, residual and the kept pre-activation 63); 64 x 128 by eight waves loses, 59 us against 55 at
+// 1536 x 1024 x 2048.
 template <int BM_, int BN_, int WM_, int WN_, int START_, int SIMD_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, START = START_, TH = 64 * WM * WN;
@@ -1197,7 +1198,8 @@ struct TileCost {
   }
 };
 constexpr TileCost kTiles[4] = {{256, 256, 1, 1.51, 2.07, 7.8}, {128, 128, 2, 0.62, 1.28, 4.0}, {64, 128, 3, 0.51, 1.14, 4.1}, {32, 128, 4, 0.43, 1.11, 2.2}};
-// the ragged products, fitted to 12 shapes with groups of random sizes, 2 % over the best choice
+// the ragged products, fitted to 12 shapes with groups of random sizes, 2 % over the best choice; their slabs take longer than
+// dense ones because what looks for the work leaves the main loop fewer registers than it needs
 constexpr TileCost kRowTiles[4] = {{256, 256, 1, 1.48, 2.14, 7.8}, {128, 128, 2, 0.81, 1.43, 4.8}, {64, 128, 3, 0.55, 1.21, 3.6}, {32, 128, 4, 0.45, 1.31, 2.0}};
 constexpr TileCost kDepthTiles[4] = {{256, 256, 1, 1.20, 2.80, 6.7}, {128, 128, 2, 1.26, 1.91, 4.4}, {64, 128, 3, 0.84, 1.54, 4.4}, {32, 128, 4, 0.73, 1.55, 2.7}};
 constexpr int kTileThreads[4] = {Tile256::TH, Tile128::TH, Tile64::TH, Tile32::TH};
